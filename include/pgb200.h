@@ -372,6 +372,67 @@ PGB_API int pgb_peer_allreduce_max_f32(float *value, void *const *peer_ctrl, int
 PGB_API int pgb_peer_allgather(const void *src, size_t bytes, void *const *peer_dst, void *const *peer_ctrl, int rank,
                                int world, void *stream);
 
+/* ---- Generation: a paged key / value cache, attention over it, logits ------------------------------------------------
+ * The reference's GPT-2 generates by recomputing every position for each new token (examples/gpt2.py:383-402); these
+ * entry points have no counterpart there.
+ *
+ * A cache is two tensors k_cache and v_cache [pages, heads, page size, head dim], f16, bf16 or int8: views with a
+ * contiguous head dim of 64 or 128 whose page, head and slot pitches are multiples of 16 bytes (so a [pages, page size,
+ * heads, head dim] array is passed as a permuted view); page sizes 16, 32, 64 and 128. An int8 cache has k_scale and
+ * v_scale, f32 [pages, heads, page size]: one scale per cached token and head. A 16-bit cache has none (NULL).
+ *
+ * The plan: rows of new tokens are packed, sequence after sequence;
+ *   q_start     int32 [sequences + 1], non-decreasing: sequence s has the rows q_start[s] .. q_start[s + 1] - 1
+ *   ctx_len     int32 [sequences]: cached tokens of each sequence, its new ones included, so that row r of sequence s stands
+ *               at position ctx_len[s] - q_start[s + 1] + r
+ *   page_table  int32 [sequences, n]: entry i is the page of positions i * page size and up. A position outside the table,
+ *               or an entry outside 0 .. pages - 1 (-1, say), has no page.
+ * They are read on the device. Rows behind the last sequence are padding: they are neither read for their values nor
+ * written. A plan can say nothing that makes a kernel reach outside the tensors it was given. */
+
+/* Stores new rows: k, v [rows, heads, head dim] (f16 or bf16, views with a contiguous head dim and 16-byte pitches). Into a
+ * 16-bit cache (of their dtype) they are copied; into an int8 cache each token's head is quantised by the rule of
+ * pgb_quantize_i8 with its own maximum: s = max(max |x|, 1e-6) / 127, q = clip(rint(x / s), -127, 127). A head with a NaN or
+ * an infinity gets the scale NaN. A position without a page is not stored. A page that is written belongs to one sequence:
+ * two rows for one slot leave it with bytes of either. */
+PGB_API int pgb_kv_write(const pgb_tensor *k, const pgb_tensor *v, const pgb_tensor *k_cache, const pgb_tensor *v_cache,
+                         const pgb_tensor *k_scale, const pgb_tensor *v_scale, const pgb_tensor *q_start,
+                         const pgb_tensor *ctx_len, const pgb_tensor *page_table, void *stream);
+
+/* Reads sequences back into packed rows: row r of k and v [rows, heads, head dim] becomes position r - kv_start[s] of the
+ * sequence s with kv_start[s] <= r < kv_start[s + 1] (kv_start as q_start above). A 16-bit cache is copied (k and v have its
+ * dtype), an int8 cache dequantised, q * s rounded once to f16, bf16 or f32. A position without a page reads as zero. */
+PGB_API int pgb_kv_read(const pgb_tensor *k_cache, const pgb_tensor *v_cache, const pgb_tensor *k_scale,
+                        const pgb_tensor *v_scale, const pgb_tensor *kv_start, const pgb_tensor *page_table, const pgb_tensor *k,
+                        const pgb_tensor *v, void *stream);
+
+/* Causal attention of the new rows over their sequences' caches, the new tokens' own keys included (pgb_kv_write comes
+ * first): out[r, h] = softmax(scale * q[r, h] . k_j) v_j over the keys j from 0 to the row's position that have a page.
+ *   q, out   [rows, q heads, head dim] f16 or bf16, views with a contiguous head dim and 16-byte pitches; q heads is a
+ *            multiple of the cache's heads, and consecutive query heads share a key head
+ *   cache    of q's dtype, or int8
+ * A row without a key gets zeros. One token per sequence or a long chunk, mixed as they come. fp32 accumulation and softmax
+ * statistics. */
+PGB_API int pgb_paged_attention(const pgb_tensor *q, const pgb_tensor *k_cache, const pgb_tensor *v_cache,
+                                const pgb_tensor *k_scale, const pgb_tensor *v_scale, const pgb_tensor *q_start,
+                                const pgb_tensor *ctx_len, const pgb_tensor *page_table, float scale, const pgb_tensor *out,
+                                void *stream);
+
+/* Logits [rows, vocabulary] shaped before a token is picked, in fp32, rounded once to the dtype (f16, bf16 or f32):
+ *   x = logits[r, v]
+ *   if v occurs in history[r, 0 .. history_len[r]):  x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   x = x - frequency[r] * n - presence[r] * (n > 0),  n = how often v occurs in history[r, prompt_len[r] .. history_len[r])
+ *   x = x + the sum of bias[r, i] over all i with bias_ids[r, i] == v
+ *   out[r, v] = bit v % 32 of mask[r, v / 32] set ? x : -inf
+ * Each part may be NULL: history [rows, n] int32 (then no penalties, lengths); history_len, prompt_len int32 [rows] (n and
+ * 0); repetition, frequency, presence f32 [rows] (1, 0, 0); bias_ids int32 and bias f32 [rows, m]; mask int32 [rows, words].
+ * Token ids outside the vocabulary are passed over. out may be logits itself. The vocabulary dim is contiguous, rows at
+ * any pitch. */
+PGB_API int pgb_logits_process(const pgb_tensor *logits, const pgb_tensor *history, const pgb_tensor *history_len,
+                               const pgb_tensor *prompt_len, const pgb_tensor *repetition, const pgb_tensor *frequency,
+                               const pgb_tensor *presence, const pgb_tensor *bias_ids, const pgb_tensor *bias,
+                               const pgb_tensor *mask, const pgb_tensor *out, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -268,6 +268,91 @@ def gemm_wait_drill(polls: int, skip_loads: bool = True) -> None:
     L.check(L.lib().pgb_gemm_wait_drill(polls, 1 if skip_loads else 0))
 
 
+# ---- generation: the paged cache, attention over it, logits -----------------------------------------------------------
+
+def _packed(ref: torch.Tensor, tensors) -> list:
+    """Descriptors of tensors (None stays None) that must lie on `ref`'s device."""
+    out = []
+    dev = ref.device
+    if dev.type != "cuda":
+        raise RuntimeError("pgb200 kernels need CUDA tensors: there is no CPU path")
+    for t in tensors:
+        if t is None:
+            out.append(None)
+            continue
+        if t.device != dev:
+            raise ValueError(f"all tensors must be on one device: {t.device} and {dev}")
+        dt = _TORCH2PGB.get(t.dtype)
+        if dt is None:
+            pgb_dtype(t.dtype)  # raises
+        es = t.element_size()
+        out.append(L.pack_tensor(t.data_ptr(), dt, t.shape, [s * es for s in t.stride()]))
+    return out
+
+
+def _call(fn, dev: torch.device, args) -> None:
+    """fn(*args, the device's current stream) with that device current."""
+    if dev.index == torch.cuda.current_device():
+        st = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if st != L.OK:
+        L.check(st)
+
+
+def kv_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, q_start: torch.Tensor, ctx_len: torch.Tensor,
+             page_table: torch.Tensor, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> None:
+    """Store new rows k, v [rows, heads, D] in a paged cache [pages, heads, page size, D]: a copy, or int8 with one scale per
+    token and head (k_scale / v_scale [pages, heads, page size] float32). q_start [B + 1], ctx_len [B] (new tokens included)
+    and page_table [B, n] are int32 on the device; a position whose table entry is no page is not stored."""
+    _call(L.lib().pgb_kv_write, k.device, _packed(k, (k, v, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len, page_table)))
+
+
+def kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_start: torch.Tensor, page_table: torch.Tensor, rows: int,
+            k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None, out_dtype=None, out=None):
+    """(k, v) [rows, heads, D]: positions 0, 1, .. of each sequence, packed from row kv_start[b] on; int8 caches are
+    dequantised to `out_dtype` (float16 by default). `out`: a pair of tensors to fill; rows behind the last sequence stay as
+    they are there (and are undefined without it)."""
+    if out is None:
+        dt = out_dtype or (torch.float16 if k_cache.dtype == torch.int8 else k_cache.dtype)
+        shape = (rows, k_cache.shape[1], k_cache.shape[3])
+        out = torch.empty(shape, dtype=dt, device=k_cache.device), torch.empty(shape, dtype=dt, device=k_cache.device)
+    elif out[0].shape[0] != rows or (out_dtype is not None and out[0].dtype != out_dtype):
+        raise ValueError("kv_read: out does not have the rows or the dtype asked for")
+    _call(L.lib().pgb_kv_read, k_cache.device, _packed(k_cache, (k_cache, v_cache, k_scale, v_scale, kv_start, page_table, *out)))
+    return out
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, q_start: torch.Tensor, ctx_len: torch.Tensor,
+                    page_table: torch.Tensor, scale: float | None = None, k_scale: torch.Tensor | None = None,
+                    v_scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of new rows q [rows, query heads, D] over their sequences' cached keys and values (their own among
+    them: `kv_write` comes first). The plan is the one of `kv_write`; rows without a key get zeros, rows behind the last
+    sequence are not written."""
+    if scale is None:
+        scale = float(q.shape[-1]) ** -0.5
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    a = _packed(q, (q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len, page_table, out))
+    a.insert(8, scale)
+    _call(L.lib().pgb_paged_attention, q.device, a)
+    return out
+
+
+def logits_process(logits: torch.Tensor, history: torch.Tensor | None = None, history_len: torch.Tensor | None = None,
+                   prompt_len: torch.Tensor | None = None, repetition: torch.Tensor | None = None, frequency: torch.Tensor | None = None,
+                   presence: torch.Tensor | None = None, bias_ids: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                   mask: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Logits [rows, vocabulary] with penalties for tokens of `history`, sparse biases added and tokens whose bit in `mask`
+    is clear set to -inf (the formula stands at pgb_logits_process). `out` may be `logits`."""
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    _call(L.lib().pgb_logits_process, logits.device,
+          _packed(logits, (logits, history, history_len, prompt_len, repetition, frequency, presence, bias_ids, bias, mask, out)))
+    return out
+
+
 class PreparedReduce:
     """A fused reduce with its descriptors and programs built once, so that a
     call is one C-ABI invocation (what the reference's `Compiled` primitive
