@@ -1,0 +1,49 @@
+// Shared by the two kernels of attention over the paged cache (paged_rows.cu, paged_chunk.cu) and their entry point
+// (paged_attention.cu).
+#pragma once
+#include "kv_cache.cuh"
+
+namespace pgb {
+
+struct PagedParams {
+  const uint8_t *q;
+  uint8_t *out;
+  int64_t q_row, q_head, o_row, o_head;  // bytes
+  int64_t rows;
+  int heads, group;  // query heads; query heads per key head
+  float c;           // scale * log2(e)
+};
+
+// Few rows per sequence: tiles of 16 rows, keys streamed once, split over a cluster. Right for any number of rows.
+int run_paged_rows(const PagedParams &a, const KvCache &c, const KvPlan &p, bool half, cudaStream_t stream);
+
+__device__ __forceinline__ float paged_ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+template <bool HALF>
+__device__ __forceinline__ uint32_t paged_pack(float lo, float hi) {
+  uint32_t r;
+  if (HALF) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Two of four int8 values (the low or the high pair of w) as exact 16-bit floats. fp16: the byte plus 128 is placed in the
+// mantissa of 1024, and 1152 taken off. bf16: its low seven bits in the mantissa of 128, less 128 or, where the sign bit
+// makes that 256, 256.
+template <bool HALF>
+__device__ __forceinline__ uint32_t paged_widen2(uint32_t w, int high) {
+  uint32_t r;
+  if (HALF) {
+    const uint32_t u = __byte_perm(w ^ 0x80808080u, 0x64646464u, high ? 0x4342 : 0x4140);
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0x64806480u));
+  } else {
+    const uint32_t u = __byte_perm(w, 0u, high ? 0x4342 : 0x4140);
+    const uint32_t a = (u & 0x007f007fu) | 0x43004300u, b = (u & 0x00800080u) | 0x43004300u;
+    asm("sub.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  }
+  return r;
+}
+
+}  // namespace pgb

@@ -1,0 +1,457 @@
+// Attention over the paged cache for few rows per sequence (decoding, speculated continuations).
+//
+// The work is reading the cache once: 16 rows of arithmetic ride on every key, so the kernel is bound by HBM, and with one
+// short sequence by latency. A work item is (16 rows, key head): the rows are consecutive tokens times the query heads that
+// share the key head. Its keys are split over the CTAs of a cluster and their four warps, 16 keys at a time.
+//   copies   each lane copies its own fragments into its own slots of shared memory with cp.async, several blocks ahead, and
+//            reads them back itself: no barrier, and the copies in flight cost no registers. A key that nobody sees (behind
+//            the context, no page) is filled with zeros, so that nothing stale meets a probability of zero.
+//   products mma.sync m16n8k16: one token of one head uses a sixteenth of it, and still the tensor pipe waits for memory. The
+//            contraction is taken in whatever order the 16-byte chunks of a row arrive (Q is held in that order), and the
+//            columns of the output likewise, so both products take their operands as they lie in memory.
+//   softmax  running maximum and sum per row in fp32; the warps' and then the CTAs' partial results are joined in shared and
+//            distributed shared memory, in a fixed order. No scratch in global memory, nothing shared between launches.
+//   int8     widened exactly to 16 bits; the key's scale multiplies its scores, the value's scale its probabilities, in fp32.
+//            For fp16 queries the scaled probabilities, whose range fp16 does not have, go in as two bf16 terms.
+#include <atomic>
+#include <string>
+
+#include "paged.cuh"
+
+namespace pgb {
+
+constexpr int kRowWarps = 4;
+
+template <int D, bool I8>
+struct RowTile {
+  static constexpr int kEs = I8 ? 1 : 2;
+  static constexpr int kKChunks = D * kEs / 64;              // 16-byte chunks of one key that a lane holds
+  static constexpr int kVBytes = D * kEs / 8;                // bytes of one value row that a lane holds
+  static constexpr int kVPiece = kVBytes < 16 ? 8 : 16;      // copied at once
+  static constexpr int kVPieces = kVBytes / kVPiece;
+  static constexpr int kK = 2 * kKChunks * 512, kV = 4 * kVPieces * 32 * kVPiece;
+  static constexpr int kStage = kK + kV + (I8 ? 128 : 0);    // 16 keys of one warp; an int8 block carries its 32 scales
+  static constexpr int kStages = D * kEs > 128 ? 3 : (D * kEs == 128 ? 4 : 6);
+  static constexpr int kWarp = kStages * kStage;
+  static constexpr int kJoin = kRowWarps * 16 * (D + 2) * 4;
+  static constexpr int kSmem = (kRowWarps * kWarp > kJoin ? kRowWarps * kWarp : kJoin) + 16 * (D + 2) * 4;
+};
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t dst, const void *src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(there ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <bool HALF>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (HALF)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+  return r;
+}
+__device__ __forceinline__ uint2 ld_shared8(uint32_t a) {
+  uint2 r;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a) : "memory");
+  return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+  uint32_t remote;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <bool HALF, int D, bool I8>
+__global__ void __launch_bounds__(kRowWarps * 32, 3) paged_rows_kernel(const __grid_constant__ PagedParams a, const __grid_constant__ KvCache c,
+                                                                       const __grid_constant__ KvPlan p, unsigned splits, unsigned tiles_per_token) {
+  using S = RowTile<D, I8>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, t = lane & 3;
+  const int rank = (int)(blockIdx.x % splits);  // of the CTA in its cluster
+  unsigned unit = blockIdx.x / splits;
+  const int kvh = (int)(unit % c.heads);
+  unit /= c.heads;
+  const int sub = (int)(unit % tiles_per_token);  // which 16 query heads, where more than that share a key head
+  const int64_t row0 = unit / tiles_per_token;
+  const int seq = kv_sequence(p, row0);
+  if (seq < 0) return;
+  const int64_t first = __ldg(p.start + seq), end = min((int64_t)__ldg(p.start + seq + 1), a.rows);
+  const int tokens = a.group >= 16 ? 1 : 16 / a.group;  // tokens of a tile
+  if ((row0 - first) % tokens) return;                 // another tile's row
+  // Row i of the tile: token i / group, query head i % group (of the 16 that start at sub * 16)
+  const int heads_here = min(a.group - sub * 16, 16);
+  const int n_tok = (int)min((int64_t)tokens, end - row0);
+  const int n_rows = n_tok * heads_here;
+  const int64_t held = (int64_t)p.width << c.log2_page;
+  const int64_t pos0 = kv_position(p, seq, row0);
+  const int64_t n_keys = max((int64_t)0, min(pos0 + n_tok, held));  // what the tile's last token sees
+  const int64_t n_blocks = (n_keys + 15) >> 4;
+
+  // Q in the order in which the chunks of K arrive: value i of this lane's D / 4 is d = 16/es * (t + 4 (i es / 16)) + ...
+  constexpr int kPer = 16 / S::kEs;  // values in a 16-byte chunk of K
+  uint32_t q[D / 16][4];
+  int64_t lim[2];  // last key that the lane's two rows see
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int i = quad + 8 * h;
+    const int tok = i / heads_here, head = i - tok * heads_here;
+    lim[h] = min(pos0 + tok, held - 1);
+    const bool in = i < n_rows;
+    if (!in) lim[h] = -1;
+    const uint8_t *src = a.q + (row0 + (in ? tok : 0)) * a.q_row + ((int64_t)kvh * a.group + sub * 16 + (in ? head : 0)) * a.q_head;
+#pragma unroll
+    for (int j = 0; j < S::kKChunks; ++j) {
+#pragma unroll
+      for (int e = 0; e < kPer; e += 8) {
+        uint4 r = make_uint4(0, 0, 0, 0);
+        if (in) r = __ldg(reinterpret_cast<const uint4 *>(src + 2 * (kPer * (t + 4 * j) + e)));
+        const int s = (j * kPer + e) / 4;
+        q[s][h] = r.x; q[s][2 + h] = r.y;
+        q[s + 1][h] = r.z; q[s + 1][2 + h] = r.w;
+      }
+    }
+  }
+  const int64_t lim_min = pos0;  // the tile's first token: keys up to here are seen by all its rows
+
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem) + warp * S::kWarp;
+  const int64_t step = (int64_t)splits * kRowWarps;
+  const int64_t block0 = (int64_t)rank * kRowWarps + warp;
+  auto page_of = [&](int64_t kb) -> int { return kb < n_blocks ? kv_page(p, c, seq, kb << 4) : -1; };
+  // Starts the copies of block kb (of the page given) into a stage. What the lane copies is what it reads.
+  auto fetch = [&](int64_t kb, int page, int stage) {
+    if (kb < n_blocks) {
+      const uint32_t dst = base + stage * S::kStage;
+      const int slot0 = (int)((kb << 4) & ((1 << c.log2_page) - 1));
+      const int there = page < 0 ? 0 : (int)min((int64_t)16, n_keys - (kb << 4));  // keys of the block that exist
+      const int64_t pg = page < 0 ? 0 : page;
+      const uint8_t *k = c.k.base + pg * c.k.page + kvh * c.k.head + slot0 * c.k.slot;
+      const uint8_t *v = c.v.base + pg * c.v.page + kvh * c.v.head + slot0 * c.v.slot;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = quad + 8 * h;
+#pragma unroll
+        for (int j = 0; j < S::kKChunks; ++j)
+          copy16(dst + ((h * S::kKChunks + j) * 32 + lane) * 16, key < there ? k + key * c.k.slot + (t + 4 * j) * 16 : c.k.base, key < there);
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int key = 2 * t + (g & 1) + 8 * (g >> 1);
+#pragma unroll
+        for (int j = 0; j < S::kVPieces; ++j) {
+          const uint32_t to = dst + S::kK + ((g * S::kVPieces + j) * 32 + lane) * S::kVPiece;
+          const uint8_t *from = key < there ? v + key * c.v.slot + (quad + 8 * j) * S::kVPiece : c.v.base;
+          if (S::kVPiece == 16) copy16(to, from, key < there);
+          else copy8(to, from, key < there);
+        }
+      }
+      if (I8 && lane < 8) {  // scales of the block: slots are contiguous, 16 of them 16-byte aligned
+        const KvPages &w = lane < 4 ? c.k : c.v;
+        const float *s = w.scale + pg * w.scale_page + kvh * w.scale_head + slot0 + (lane & 3) * 4;
+        copy16(dst + S::kK + S::kV + lane * 16, page < 0 ? w.scale : s, page >= 0);
+      }
+    }
+    copy_commit();  // empty groups keep the count
+  };
+
+  float o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+  int pages[S::kStages];  // of the blocks under way
+#pragma unroll
+  for (int i = 0; i < S::kStages; ++i) pages[i] = page_of(block0 + i * step);
+#pragma unroll
+  for (int i = 0; i < S::kStages - 1; ++i) fetch(block0 + i * step, pages[i], i);
+  int stage = 0;
+  for (int64_t kb = block0; kb < n_blocks; kb += step) {
+    const int page = pages[0];
+    fetch(kb + (S::kStages - 1) * step, pages[S::kStages - 1], stage == 0 ? S::kStages - 1 : stage - 1);
+#pragma unroll
+    for (int i = 0; i + 1 < S::kStages; ++i) pages[i] = pages[i + 1];
+    pages[S::kStages - 1] = page_of(kb + S::kStages * step);
+    copy_wait<S::kStages - 1>();
+    if (I8) __syncwarp();  // the scales were copied by other lanes
+    const uint32_t src = base + stage * S::kStage;
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
+
+    float s[2][4] = {};  // keys quad-wise: [h][0..1] row quad, [h][2..3] row quad + 8; keys 2t, 2t + 1 of half h
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int j = 0; j < S::kKChunks; ++j) {
+        const uint4 r = ld_shared16(src + ((h * S::kKChunks + j) * 32 + lane) * 16);
+        if constexpr (I8) {
+          const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mma16816<HALF>(s[h], q[4 * j + e], paged_widen2<HALF>(w[e], 0), paged_widen2<HALF>(w[e], 1));
+        } else {
+          mma16816<HALF>(s[h], q[2 * j], r.x, r.y);
+          mma16816<HALF>(s[h], q[2 * j + 1], r.z, r.w);
+        }
+      }
+    }
+    float vs[4];
+    {
+      float ks[4] = {a.c, a.c, a.c, a.c};
+      if constexpr (I8) {
+        const uint32_t at = src + S::kK + S::kV + 8 * t;
+        const uint2 k0 = ld_shared8(at), k1 = ld_shared8(at + 32), v0 = ld_shared8(at + 64), v1 = ld_shared8(at + 96);
+        ks[0] *= __uint_as_float(k0.x); ks[1] *= __uint_as_float(k0.y); ks[2] *= __uint_as_float(k1.x); ks[3] *= __uint_as_float(k1.y);
+        vs[0] = __uint_as_float(v0.x); vs[1] = __uint_as_float(v0.y); vs[2] = __uint_as_float(v1.x); vs[3] = __uint_as_float(v1.y);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[h][e] *= ks[2 * h + (e & 1)];
+    }
+    const int64_t key0 = kb << 4;
+    if (key0 + 15 > lim_min || page < 0) {  // warp-uniform
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int64_t key = key0 + 8 * h + 2 * t + (e & 1);
+          if (key > lim[e >> 1] || page < 0) s[h][e] = -INFINITY;
+          // a slot behind the context has a stale scale: its probability of zero must meet a number
+          if (I8 && e < 2 && (key >= n_keys || page < 0)) vs[2 * h + e] = 0.f;
+        }
+    }
+    float mx[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      mx[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+    }
+    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {  // rare once the largest scores have been met
+      float alpha[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float mn = fmaxf(m[r], mx[r]);
+        alpha[r] = mn == -INFINITY ? 1.f : paged_ex2(m[r] - mn);
+        m[r] = mn;
+        l[r] *= alpha[r];
+      }
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        o[i][0] *= alpha[0]; o[i][1] *= alpha[0];
+        o[i][2] *= alpha[1]; o[i][3] *= alpha[1];
+      }
+    }
+    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[h][e] = paged_ex2(s[h][e] - ref[e >> 1]);
+        l[e >> 1] += s[h][e];
+      }
+    // The probabilities as the A operand of the second product: the accumulator's layout is the operand's.
+    constexpr bool kTwoTerms = I8 && HALF;
+    constexpr bool kPHalf = HALF && !I8;
+    uint32_t pa[4], pb[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float x = s[h][2 * r], y = s[h][2 * r + 1];
+        if (I8) { x *= vs[2 * h]; y *= vs[2 * h + 1]; }
+        pa[2 * h + r] = paged_pack<kPHalf>(x, y);
+        if (kTwoTerms) {
+          const float xr = x - __uint_as_float(pa[2 * h + r] << 16), yr = y - __uint_as_float(pa[2 * h + r] & 0xffff0000u);
+          pb[2 * h + r] = paged_pack<false>(xr, yr);
+        }
+      }
+    const uint32_t vsrc = src + S::kK + lane * S::kVPiece;
+    auto value_words = [&](int g, int j) -> uint4 {
+      const uint32_t at = vsrc + (g * S::kVPieces + j) * 32 * S::kVPiece;
+      if constexpr (S::kVPiece == 16) return ld_shared16(at);
+      else { const uint2 r = ld_shared8(at); return make_uint4(r.x, r.y, 0, 0); }
+    };
+#pragma unroll
+    for (int j = 0; j < S::kVPieces; ++j) {
+      const uint4 r0 = value_words(0, j), r1 = value_words(1, j), r2 = value_words(2, j), r3 = value_words(3, j);
+      const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w}, w2[4] = {r2.x, r2.y, r2.z, r2.w}, w3[4] = {r3.x, r3.y, r3.z, r3.w};
+      constexpr int kWords = S::kVPiece / 4;
+#pragma unroll
+      for (int e = 0; e < kWords; ++e) {
+        if constexpr (I8) {
+          // bytes of two keys interleaved, then each pair widened: value d of keys 2t and 2t + 1 in one register
+          const uint32_t lo01 = __byte_perm(w0[e], w1[e], 0x5140), hi01 = __byte_perm(w0[e], w1[e], 0x7362);
+          const uint32_t lo23 = __byte_perm(w2[e], w3[e], 0x5140), hi23 = __byte_perm(w2[e], w3[e], 0x7362);
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const uint32_t b0 = paged_widen2<kPHalf>(d < 2 ? lo01 : hi01, d & 1), b1 = paged_widen2<kPHalf>(d < 2 ? lo23 : hi23, d & 1);
+            float(&acc)[4] = o[j * kWords * 4 + 4 * e + d];
+            mma16816<kPHalf>(acc, pa, b0, b1);
+            if (kTwoTerms) mma16816<kPHalf>(acc, pb, b0, b1);
+          }
+        } else {
+          mma16816<HALF>(o[j * 8 + 2 * e], pa, __byte_perm(w0[e], w1[e], 0x5410), __byte_perm(w2[e], w3[e], 0x5410));
+          mma16816<HALF>(o[j * 8 + 2 * e + 1], pa, __byte_perm(w0[e], w1[e], 0x7632), __byte_perm(w2[e], w3[e], 0x7632));
+        }
+      }
+    }
+  }
+  copy_wait<0>();
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+  }
+  __syncthreads();  // every warp is done with its stages: the memory now holds partial results
+
+  // [warp][row][D], then m and l of [warp][row]. Accumulator i of a lane's columns 2t, 2t + 1 is value kCol * (2t + e) + i of
+  // its piece (kCol values a column).
+  float *part = reinterpret_cast<float *>(smem);
+  float *part_m = part + kRowWarps * 16 * D, *part_l = part_m + kRowWarps * 16;
+  constexpr int kCol = S::kVPiece / S::kEs;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int row = quad + 8 * r;
+    if (row < n_rows) {
+      float *dst = part + (warp * 16 + row) * D;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const int piece = i / kCol, d = piece * 8 * kCol + i % kCol;
+        dst[d + kCol * (2 * t)] = o[i][2 * r];
+        dst[d + kCol * (2 * t + 1)] = o[i][2 * r + 1];
+      }
+      if (t == 0) {
+        part_m[warp * 16 + row] = m[r];
+        part_l[warp * 16 + row] = l[r];
+      }
+    }
+  }
+  __syncthreads();
+  // the warps of this CTA, and behind a cluster barrier its CTAs
+  float *mine = reinterpret_cast<float *>(smem + S::kSmem) - 16 * (D + 2), *mine_m = mine + 16 * D, *mine_l = mine_m + 16;
+  auto write = [&](int row, int d, float x) {  // two neighbours are written by two lanes
+    const int tok = row / heads_here, head = row - tok * heads_here;
+    uint8_t *out = a.out + (row0 + tok) * a.o_row + ((int64_t)kvh * a.group + sub * 16 + head) * a.o_head;
+    const float y = __shfl_down_sync(__activemask(), x, 1);
+    if (!(d & 1)) *reinterpret_cast<uint32_t *>(out + 2 * d) = paged_pack<HALF>(x, y);
+  };
+  for (int i = threadIdx.x; i < n_rows * D; i += kRowWarps * 32) {
+    const int row = i / D, d = i % D;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) mm = fmaxf(mm, part_m[w * 16 + row]);
+    float x = 0.f, sum = 0.f;
+    if (mm != -INFINITY) {
+#pragma unroll
+      for (int w = 0; w < kRowWarps; ++w) {
+        const float e = paged_ex2(part_m[w * 16 + row] - mm);
+        x += part[(w * 16 + row) * D + d] * e;
+        sum += part_l[w * 16 + row] * e;
+      }
+    }
+    if (splits == 1) {
+      write(row, d, mm == -INFINITY ? 0.f : x / sum);
+    } else {
+      mine[row * D + d] = x;
+      if (d == 0) { mine_m[row] = mm; mine_l[row] = sum; }
+    }
+  }
+  if (splits == 1) return;
+  cluster_sync();
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(mine), at_m = (uint32_t)__cvta_generic_to_shared(mine_m), at_l = (uint32_t)__cvta_generic_to_shared(mine_l);
+  // each CTA writes its share of the outputs: 32 of them at a time
+  for (int i = (rank * kRowWarps + warp) * 32 + lane; i < n_rows * D; i += splits * kRowWarps * 32) {
+    const int row = i / D, d = i % D;
+    float mm = -INFINITY;
+    for (int s = 0; s < splits; ++s) mm = fmaxf(mm, ld_cluster(at_m + 4 * row, s));
+    float x = 0.f, sum = 0.f;
+    if (mm != -INFINITY) {
+      for (int s = 0; s < splits; ++s) {
+        const float e = paged_ex2(ld_cluster(at_m + 4 * row, s) - mm);
+        x += ld_cluster(at + 4 * i, s) * e;
+        sum += ld_cluster(at_l + 4 * row, s) * e;
+      }
+    }
+    write(row, d, mm == -INFINITY ? 0.f : x / sum);
+  }
+  cluster_sync();  // nobody's shared memory goes away while it is read
+}
+
+template <bool HALF, int D, bool I8>
+static int launch(const PagedParams &a, const KvCache &c, const KvPlan &p, int splits, int tiles_per_token, int64_t units, cudaStream_t stream) {
+  using S = RowTile<D, I8>;
+  const auto kernel = paged_rows_kernel<HALF, D, I8>;
+  // the attribute belongs to the device: set once on each, again where two threads meet
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    if (e != cudaSuccess) {
+      set_error(std::string("paged_attention: cannot raise the shared-memory limit: ") + cudaGetErrorString(e));
+      return PGB_ERR_CUDA;
+    }
+    if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * splits));
+  cfg.blockDim = dim3(kRowWarps * 32);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, c, p, (unsigned)splits, (unsigned)tiles_per_token);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_error(std::string("paged_rows_kernel: ") + cudaGetErrorString(e));
+    return PGB_ERR_CUDA;
+  }
+  count_launch();
+  return PGB_OK;
+}
+
+int run_paged_rows(const PagedParams &a, const KvCache &c, const KvPlan &p, bool half, cudaStream_t stream) {
+  const int tiles_per_token = (a.group + 15) / 16;
+  const int64_t units = a.rows * tiles_per_token * c.heads;
+  // As many CTAs per item as leave no SM idle, up to a portable cluster; not more than have a block of keys for each warp.
+  int splits = 1;
+  const int64_t blocks = ((int64_t)p.width << c.log2_page) / 16;
+  while (splits < 8 && units * splits < 4LL * sm_count() && blocks > (int64_t)splits * kRowWarps) splits *= 2;
+  if (units * splits > 2147483647LL) {
+    set_error("paged_attention: too many rows for one launch");
+    return PGB_ERR_UNSUPPORTED;
+  }
+  const bool i8 = c.dtype == PGB_I8;
+#define PGB_ROWS(H, D, Q) return launch<H, D, Q>(a, c, p, splits, tiles_per_token, units, stream)
+  if (half) {
+    if (c.head_dim == 64) { if (i8) PGB_ROWS(true, 64, true); PGB_ROWS(true, 64, false); }
+    if (i8) PGB_ROWS(true, 128, true);
+    PGB_ROWS(true, 128, false);
+  }
+  if (c.head_dim == 64) { if (i8) PGB_ROWS(false, 64, true); PGB_ROWS(false, 64, false); }
+  if (i8) PGB_ROWS(false, 128, true);
+  PGB_ROWS(false, 128, false);
+#undef PGB_ROWS
+}
+
+}  // namespace pgb
