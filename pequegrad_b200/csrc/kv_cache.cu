@@ -98,7 +98,8 @@ int kv_parse_plan(const char *what, const pgb_tensor *start, const pgb_tensor *c
   if (table->ndim != 2 || table->shape[0] != B) return fail(PGB_ERR_INVALID_ARG, what, "the page table must be [sequences, pages of a sequence]");
   if (table->shape[1] > 1 && table->stride_bytes[1] != 4) return fail(PGB_ERR_INVALID_ARG, what, "the rows of the page table must be contiguous");
   if (table->stride_bytes[0] < 0 || table->stride_bytes[0] % 4) return fail(PGB_ERR_INVALID_ARG, what, "bad stride in the page table");
-  if (B > 1000000 || table->shape[1] > (1 << 24)) return fail(PGB_ERR_UNSUPPORTED, what, "too many sequences or pages");
+  // positions are 32-bit numbers: 2^23 pages of at most 128 tokens
+  if (B > 1000000 || table->shape[1] > (1 << 23)) return fail(PGB_ERR_UNSUPPORTED, what, "too many sequences or pages");
   if (B && (!start->data || (ctx && !ctx->data) || (table->shape[1] && !table->data))) return fail(PGB_ERR_INVALID_ARG, what, "null plan");
   for (const pgb_tensor *t : {start, ctx, table})
     if (t && (reinterpret_cast<uintptr_t>(t->data) & 3)) return fail(PGB_ERR_INVALID_ARG, what, "row offsets, lengths and the page table must be 4-byte aligned");

@@ -16,6 +16,9 @@ struct PagedParams {
 
 // Few rows per sequence: tiles of 16 rows, keys streamed once, split over a cluster. Right for any number of rows.
 int run_paged_rows(const PagedParams &a, const KvCache &c, const KvPlan &p, bool half, cudaStream_t stream);
+// Many rows per sequence: tiles of 256 rows on the tensor cores. False where the pages cannot be addressed by TMA, or there
+// are none: nothing was launched. Right for any number of rows.
+bool run_paged_chunk(const PagedParams &a, const KvCache &c, const KvPlan &p, bool half, cudaStream_t stream, int *status);
 
 __device__ __forceinline__ float paged_ex2(float x) {
   float r;

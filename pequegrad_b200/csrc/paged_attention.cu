@@ -46,6 +46,8 @@ static int paged_attention(const pgb_tensor *q, const pgb_tensor *k_cache, const
   a.c = scale * 1.4426950408889634f;
   if (a.rows == 0 || p.n_seq == 0) return PGB_OK;
   if (c.n_pages == 0) p.width = 0;  // no page at all: no key for anyone, and nothing to point a load at
+  // Rows of a sequence on average, times the query heads that share a key: what rides on one pass over the keys.
+  if (a.rows * a.group > 32LL * p.n_seq && run_paged_chunk(a, c, p, q->dtype == PGB_F16, stream, &st)) return st;
   return run_paged_rows(a, c, p, q->dtype == PGB_F16, stream);
 }
 

@@ -1,0 +1,910 @@
+// Attention over the paged cache for chunks of new tokens, on the 5th-generation tensor cores.
+//
+// Work item = (key head, 256 packed rows): the rows of a sequence are its new tokens times the query heads that share the
+// key head (token t, head g is row t * group + g), so grouped heads fill the tiles whatever their number. The two halves of
+// 128 rows, A and B, meet every block of 128 keys together: a block is fetched, and for an int8 cache widened, once for
+// both. One CTA per SM walks its share of the items; where there are fewer items than SMs, a cluster of CTAs splits the
+// keys of one item and joins the partial results in distributed shared memory.
+//   warps 0-3, 4-7  softmax of A and of B: thread = row. Scores from tensor memory into registers, mask, running maximum,
+//                   exponentials, row sum, probabilities as 16-bit pairs back into tensor memory. O is rescaled there only when
+//                   a row's maximum outgrew its reference by 2^8.
+//   warps 8-11      keys and values. 16 bits: one warp issues a TMA box per page (an index that is no page reads as zeros).
+//                   int8: each warp brings 32 keys a block into a raw ring with cp.async, widens them exactly to 16 bits and
+//                   stores them as the tiles TMA would have written; scales go to the softmax warps through a small ring.
+//   warp 12         tensor memory; issues the MMAs (one lane)
+//   warps 13-15     Q rows, by cp.async into the swizzled tiles
+// Tensor memory: S_A [0, 128), S_B [128, 256), O_A, O_B behind them. With head dim 64 there is room for P beside S, and the
+// scores of the next block are computed under the softmax of this one; with 128 P takes the place of S, and the two halves
+// keep the tensor pipe and the exponentials busy in turn.
+// int8 scales: the key's multiplies its scores, the value's its probabilities, both in fp32. In fp16 the product's range is
+// kept by a common power of two per block, which joins the exponents' reference and leaves O / l as it is.
+// Masked places: a score that is left out is -inf by selection, its probability zero. Value rows behind the context are
+// zeroed in shared memory, and values of new tokens that some rows must not see are cleared of NaN and infinities there;
+// the rows that do see such a token get them back in the epilogue.
+// Every wait is bounded; one that runs out sets the device error word and the CTA drains.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <string>
+
+#include "attention_ptx.cuh"
+#include "paged.cuh"
+
+namespace pgb {
+
+constexpr int kChunkRows = 256;     // of an item
+constexpr int kChunkThreads = 512;
+constexpr uint32_t kChunkPolls = 1u << 20;
+constexpr float kChunkLazy = 8.0f;  // log2 of the largest probability before a row's reference moves
+constexpr int kScaleSlots = 4;
+
+template <int D, bool I8>
+struct ChunkTile {
+  static constexpr bool kAhead = D == 64;  // P beside S: the next scores are computed ahead
+  static constexpr int kQ = kChunkRows * D * 2, kKV = 128 * D * 2, kRaw = 128 * D * 2;  // raw: K and V of a block, int8
+  static constexpr int kStages = I8 ? (D == 64 ? 2 : 1) : (D == 64 ? 3 : 2);
+  static constexpr int kRawStages = I8 ? (D == 64 ? 3 : 2) : 0;
+  static constexpr int kRing = 2 * kStages * kKV + kRawStages * kRaw;
+  static constexpr int kScales = I8 ? kScaleSlots * (2 * 128 + 4) * 4 : 0;
+  static constexpr int kMl = 2 * kChunkRows * 4;
+  static constexpr int kSmem = kQ + kRing + kScales + kMl + 512 /*barriers*/ + 1024 /*alignment*/;
+  static_assert(kRing >= kChunkRows * D * 4, "the partial results of a split item take the place of the rings");
+  static_assert(kSmem <= 232448, "shared memory of one SM");
+};
+
+struct ChunkParams {
+  PagedParams a;
+  KvCache c;
+  KvPlan p;
+  int n_tiles;  // bound on the tiles of all sequences
+  int splits;
+  int *err;
+  uint32_t polls;
+  int skip_loads;
+};
+
+struct ChunkItem {
+  int seq, head;
+  int token, sub;        // of the first packed row: row of q, query head of the group
+  int rows;              // packed rows of the item, at most 256
+  int pos;               // position of that token
+  int n_keys;            // keys that the item's last row sees
+  int first_seen;        // last key that the item's first row sees
+  int lo;                // first block of this CTA
+  int steps, blocks[2];  // blocks of this CTA; of each half
+};
+
+struct ChunkCursor {
+  int seq0 = 0, base = 0;
+};
+
+// Tile `t` of the list of all sequences' tiles, found by a warp: sequences 32 at a time. Tiles are asked for in ascending
+// order, so the search resumes where it stopped. False past the last tile.
+__device__ __forceinline__ bool chunk_item(const ChunkParams &P, int id, int rank, ChunkCursor &cur, ChunkItem &it) {
+  const int lane = threadIdx.x & 31;
+  const int t = id / P.c.heads;
+  it.head = id - t * P.c.heads;
+  for (; cur.seq0 < P.p.n_seq; cur.seq0 += 32) {
+    const int s = cur.seq0 + lane;
+    int64_t start = 0, n = 0;
+    if (s < P.p.n_seq) {
+      start = __ldg(P.p.start + s);
+      n = min((int64_t)__ldg(P.p.start + s + 1), P.a.rows) - start;
+      if (n < 0 || start < 0) n = 0;  // offsets that make no sense hold no rows
+    }
+    const int64_t packed = n * P.a.group;
+    const int tiles = (int)((packed + kChunkRows - 1) / kChunkRows);
+    int sum = tiles;
+#pragma unroll
+    for (int k = 1; k < 32; k <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, k);
+      if (lane >= k) sum += up;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, t < cur.base + sum);
+    if (!hit) {
+      cur.base += __shfl_sync(0xffffffffu, sum, 31);
+      continue;
+    }
+    const int src = __ffs(hit) - 1;
+    const int before = cur.base + __shfl_sync(0xffffffffu, sum - tiles, src);
+    n = __shfl_sync(0xffffffffu, n, src);
+    it.seq = cur.seq0 + src;
+    start = __shfl_sync(0xffffffffu, start, src);
+    const int64_t row0 = (int64_t)(t - before) * kChunkRows, tok0 = row0 / P.a.group;
+    it.token = (int)(start + tok0);
+    it.sub = (int)(row0 - tok0 * P.a.group);
+    it.rows = (int)min((int64_t)kChunkRows, n * P.a.group - row0);
+    const int held = P.p.width << P.c.log2_page;  // at most 2^30
+    it.pos = (int)max(kv_position(P.p, it.seq, it.token), -((int64_t)1 << 31));
+    auto keys = [&](int row) { return max(0, min(held, it.pos + (it.sub + row) / P.a.group + 1)); };
+    it.first_seen = keys(0) - 1;
+    it.n_keys = keys(it.rows - 1);
+    const int n_a = (keys(min(it.rows, 128) - 1) + 127) >> 7, n_all = (it.n_keys + 127) >> 7;
+    it.lo = n_all * rank / P.splits;
+    it.steps = n_all * (rank + 1) / P.splits - it.lo;
+    it.blocks[0] = max(0, min(it.steps, n_a - it.lo));
+    it.blocks[1] = it.rows > 128 ? it.steps : 0;
+    return true;
+  }
+  return false;
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t ua, ub, ud;
+  memcpy(&ua, &a, 8); memcpy(&ub, &b, 8);
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(ud) : "l"(ua), "l"(ub));
+  float2 d;
+  memcpy(&d, &ud, 8);
+  return d;
+}
+__device__ __forceinline__ void chunk_copy16(uint32_t dst, const void *src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ float chunk_peer(uint32_t addr, uint32_t rank) {
+  uint32_t remote;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 chunk_peer4(uint32_t addr, uint32_t rank) {
+  uint32_t remote;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
+  return v;
+}
+__device__ __forceinline__ void chunk_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// exponent all ones in either half of a word of two 16-bit floats
+template <bool HALF>
+__device__ __forceinline__ bool not_finite2(uint32_t w) {
+  constexpr uint32_t e = HALF ? 0x7c00u : 0x7f80u;
+  return (w & e) == e || ((w >> 16) & e) == e;
+}
+template <bool HALF>
+__device__ __forceinline__ float half_of(uint32_t w, int hi) {
+  const uint32_t u = hi ? w >> 16 : w & 0xffffu;
+  if (HALF) return __half2float(__ushort_as_half((unsigned short)u));
+  return __uint_as_float(u << 16);
+}
+
+template <bool HALF, int D, bool I8>
+__global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                       const __grid_constant__ ChunkParams P) {
+  using S = ChunkTile<D, I8>;
+  constexpr int kKind = GEMM_F16;  // kind::f16 serves both 16-bit types; the descriptor tells them apart
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t *q_s = smem;                          // [half][d / 64][128 rows][128 bytes]
+  uint8_t *k_s = q_s + S::kQ;                   // [stage][d / 64][128 keys][128 bytes]
+  uint8_t *v_s = k_s + S::kStages * S::kKV;
+  uint8_t *raw_s = v_s + S::kStages * S::kKV;   // [stage][K, V][128 keys][D bytes]
+  float *scale_s = reinterpret_cast<float *>(raw_s + S::kRawStages * S::kRaw);  // [slot][128 of K, 128 of V, 4 maxima]
+  float *ml_s = scale_s + S::kScales / 4;       // [m, l][256]
+  uint64_t *bars = reinterpret_cast<uint64_t *>(ml_s + 2 * kChunkRows);
+  uint64_t *q_full = bars, *q_empty = bars + 1;
+  uint64_t *k_full = bars + 2, *k_empty = k_full + 4, *v_full = k_empty + 4, *v_empty = v_full + 4;  // [kStages]
+  uint64_t *sc_full = v_empty + 4, *sc_empty = sc_full + kScaleSlots;
+  uint64_t *s_full = sc_empty + kScaleSlots, *s_free = s_full + 2, *p_full = s_free + 2, *pv_done = p_full + 2;  // [half]
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(pv_done + 2);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  int *dead = const_cast<int *>(abort_flag) + 1;
+  volatile int *poison = const_cast<volatile int *>(abort_flag) + 2;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = P.splits > 1 ? (int)(blockIdx.x % P.splits) : 0;
+  const int n_items = P.n_tiles * P.c.heads;
+  // one item per cluster, or every gridDim.x-th
+  const int id0 = (int)blockIdx.x / P.splits, id_step = P.splits > 1 ? n_items : (int)gridDim.x;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 3);
+    mbar_init(q_empty, 1);
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(&k_full[s], I8 ? 4 : 1);
+      mbar_init(&v_full[s], I8 ? 4 : 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int s = 0; s < kScaleSlots; ++s) {
+      mbar_init(&sc_full[s], 4);
+      mbar_init(&sc_empty[s], 8);
+    }
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(&s_full[h], 1);
+      mbar_init(&s_free[h], 4);
+      mbar_init(&p_full[h], 4);
+      mbar_init(&pv_done[h], 1);
+    }
+    *abort_flag = 0;
+    *poison = 0;
+    *dead = *(volatile int *)P.err != 0;  // an earlier wait ran out and nobody has cleared the word: do nothing
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 12) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const bool run = *dead == 0;
+
+  // last key that a row of the item sees
+  auto last_seen = [&](const ChunkItem &it, int row) -> int {
+    return min(it.pos + (it.sub + min(row, it.rows - 1)) / P.a.group, (P.p.width << P.c.log2_page) - 1);
+  };
+  auto out_row = [&](const ChunkItem &it, int row) -> uint8_t * {
+    const int pr = it.sub + row, tok = pr / P.a.group;
+    return P.a.out + ((int64_t)it.token + tok) * P.a.o_row + ((int64_t)it.head * P.a.group + (pr - tok * P.a.group)) * P.a.o_head;
+  };
+  // Sixteen columns of a row of O from tensor memory, and, rarely, what was cleared from the values it sees given back.
+  auto load_o = [&](const ChunkItem &it, uint32_t o_addr, int q4, bool any, bool seen, bool slow, int lim, float (&o)[16]) {
+    if (any) {
+      uint32_t r[16];
+      tmem_ld16_issue(o_addr + q4 * 16, r);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i] = seen ? __uint_as_float(r[i]) : 0.f;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i] = 0.f;
+    }
+    if (slow) {
+      const int end = min(min(lim + 1, it.n_keys), (it.lo + it.steps) << 7);
+      for (int key = max(it.first_seen + 1, it.lo << 7); key < end; ++key) {
+        const int page = kv_page(P.p, P.c, it.seq, key);
+        if (page < 0) continue;
+        const int sl = key & ((1 << P.c.log2_page) - 1);
+        const uint32_t *v = reinterpret_cast<const uint32_t *>(P.c.v.base + page * P.c.v.page + it.head * P.c.v.head + sl * P.c.v.slot) + q4 * 8;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float x = half_of<HALF>(v[i >> 1], i & 1);
+          if (!(fabsf(x) <= 3.4028234e38f)) o[i] += x;
+        }
+      }
+    }
+  };
+  // a wait of the whole warp; `role` goes into the error word
+  auto wait = [&](uint64_t *bar, uint32_t parity, int role) -> bool {
+    const bool ok = __all_sync(0xffffffffu, attn_wait(bar, parity, abort_flag, P.polls));
+    if (!ok && lane == 0) {
+      *abort_flag = 1;
+      atomicCAS(P.err, 0, (role << 16) | (int)(blockIdx.x & 0xffff));
+    }
+    return ok;
+  };
+  // 128 launch registers a thread are dealt out anew: 184 + 184 + 64 + 80 = 4 * 128
+  if (!run) {
+  } else if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp > 12) {
+    // ---- Q: 96 lanes, 16-byte pieces; rows that do not exist are zeros --------------------------------------------
+    ChunkCursor cur;
+    ChunkItem it;
+    uint32_t n = 0;
+    for (int id = id0; id < n_items && !P.skip_loads && chunk_item(P, id, rank, cur, it); id += id_step) {
+      if (it.steps == 0) continue;
+      if (!wait(q_empty, (n & 1) ^ 1, 32)) break;
+      ++n;
+      constexpr int kUnits = D / 8;
+      for (int i = (warp - 13) * 32 + lane; i < kChunkRows * kUnits; i += 96) {
+        const int r = i / kUnits, u = i % kUnits;
+        const bool in = r < it.rows;
+        const int pr = it.sub + (in ? r : 0), tok = pr / P.a.group, g = pr - tok * P.a.group;
+        const uint8_t *src = P.a.q + ((int64_t)it.token + tok) * P.a.q_row + ((int64_t)it.head * P.a.group + g) * P.a.q_head + u * 16;
+        const uint32_t dst = smem_u32(q_s) + (r >> 7) * (S::kQ / 2) + (u >> 3) * 16384 + (r & 127) * 128 + (((u & 7) ^ (r & 7)) << 4);
+        chunk_copy16(dst, src, in);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    } else {
+    // ---- MMA ------------------------------------------------------------------------------------------------------
+    const uint32_t idesc_s = attn_idesc(HALF, false, 128), idesc_pv = attn_idesc(HALF, true, D);
+    const uint32_t col_p[2] = {S::kAhead ? 384u : 0u, S::kAhead ? 448u : 128u}, col_o[2] = {256u, 256u + D};
+    ChunkCursor s_cur, cur;
+    ChunkItem s_it, it;
+    int s_id = id0, s_j = 0;
+    bool s_more = false;
+    auto s_seek = [&]() {  // the next item with blocks for this CTA
+      for (; s_id < n_items; s_id += id_step) {
+        if (!chunk_item(P, s_id, rank, s_cur, s_it)) break;
+        if (s_it.steps > 0) { s_more = true; return; }
+      }
+      s_more = false;
+    };
+    s_seek();
+    uint32_t s_g = 0, s_items = 0, s_n[2] = {0, 0};
+    // scores of half h in the step of the S cursor
+    auto issue_s = [&](int h) -> bool {
+      if (s_j >= s_it.blocks[h]) return true;
+      const uint32_t ks = s_g % S::kStages;
+      if (S::kAhead && !wait(&s_free[h], (s_n[h] & 1) ^ 1, 36)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * 16384;
+          tc_mma<kKind>(tmem + h * 128, make_kmajor_sw128_desc(smem_u32(q_s) + h * (S::kQ / 2) + off) + 2 * (kk & 3),
+                        make_kmajor_sw128_desc(smem_u32(k_s) + ks * S::kKV + off) + 2 * (kk & 3), idesc_s, kk != 0);
+        }
+        tc_commit(&s_full[h]);
+      }
+      __syncwarp();
+      ++s_n[h];
+      return true;
+    };
+    auto s_operands = [&]() -> bool {
+      if (s_j == 0 && !wait(q_full, s_items & 1, 34)) return false;
+      return wait(&k_full[s_g % S::kStages], (s_g / S::kStages) & 1, 35);
+    };
+    auto s_next = [&]() {
+      if (lane == 0) {
+        tc_commit(&k_empty[s_g % S::kStages]);
+        if (s_j + 1 == s_it.steps) tc_commit(q_empty);
+      }
+      __syncwarp();
+      ++s_g;
+      if (++s_j == s_it.steps) {
+        ++s_items;
+        s_j = 0;
+        s_id += id_step;
+        s_seek();
+      }
+    };
+    bool ok = true;
+    if (s_more) {
+      ok = s_operands() && issue_s(0) && issue_s(1);
+      if (ok) s_next();
+    }
+    uint32_t g = 0, n[2] = {0, 0};
+    for (int id = id0; id < n_items && ok && chunk_item(P, id, rank, cur, it); id += id_step) {
+      for (int j = 0; j < it.steps && ok; ++j, ++g) {
+        const uint32_t vs = g % S::kStages;
+        auto issue_pv = [&](int h) -> bool {
+          if (j >= it.blocks[h]) return true;
+          if (!wait(&p_full[h], n[h] & 1, 37)) return false;
+          if (!wait(&v_full[vs], (g / S::kStages) & 1, 38)) return false;
+          tc_fence_after();
+          if (lane == 0) {
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)  // 16 keys per MMA: 8 columns of P, 16 rows of V
+              tc_mma_ts(tmem + col_o[h], tmem + col_p[h] + kk * 8, make_mnmajor_sw128_desc(smem_u32(v_s) + vs * S::kKV + kk * 2048, 16384), idesc_pv, (j | kk) != 0);
+            tc_commit(&pv_done[h]);
+          }
+          __syncwarp();
+          ++n[h];
+          return true;
+        };
+        if (S::kAhead) {
+          if (s_more) {
+            ok = s_operands() && issue_s(0) && issue_s(1);
+            if (ok) s_next();
+          }
+          ok = ok && issue_pv(0) && issue_pv(1);
+        } else {
+          // P lies where the next scores go: they wait for the product that reads it
+          const bool more = s_more;
+          for (int h = 0; h < 2 && ok; ++h) {
+            ok = issue_pv(h);
+            if (ok && more) {
+              if (h == 0) ok = s_operands();
+              if (ok && n[h] > 0) ok = wait(&pv_done[h], (n[h] - 1) & 1, 39);
+              ok = ok && issue_s(h);
+            }
+          }
+          if (ok && more) s_next();
+        }
+        if (ok && lane == 0) tc_commit(&v_empty[vs]);
+        __syncwarp();
+      }
+    }
+    }
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    // ---- keys and values --------------------------------------------------------------------------------------------
+    ChunkCursor cur;
+    ChunkItem it;
+    uint32_t g = 0;
+    bool ok = !P.skip_loads;
+    if constexpr (!I8) {
+      if (warp == 8) {
+        const int per = 128 >> P.c.log2_page;  // pages of a block, a lane each
+        for (int id = id0; id < n_items && ok && chunk_item(P, id, rank, cur, it); id += id_step) {
+          auto page_of = [&](int j) -> int {
+            const int pos = ((it.lo + j) << 7) + (lane << P.c.log2_page);
+            const int page = lane < per && pos < it.n_keys ? kv_page(P.p, P.c, it.seq, pos) : -1;
+            return page < 0 ? P.c.n_pages : page;  // out of the tensor's range: zeros
+          };
+          int page = it.steps > 0 ? page_of(0) : 0;
+          for (int j = 0; j < it.steps && ok; ++j, ++g) {
+            const int next = j + 1 < it.steps ? page_of(j + 1) : 0;
+            const uint32_t st = g % S::kStages, ph = ((g / S::kStages) & 1) ^ 1;
+            const int box = 128 << P.c.log2_page;  // bytes of a page's 64 columns
+            for (int kv = 0; kv < 2 && ok; ++kv) {
+              uint64_t *full = kv ? &v_full[st] : &k_full[st];
+              ok = wait(kv ? &v_empty[st] : &k_empty[st], ph, 33);
+              if (!ok) break;
+              if (lane == 0) mbar_expect_tx(full, S::kKV);
+              __syncwarp();
+              if (lane < per) {
+                uint8_t *dst = (kv ? v_s : k_s) + st * S::kKV + lane * box;
+#pragma unroll
+                for (int d = 0; d < D / 64; ++d) tma_load_4d(dst + d * 16384, kv ? &map_v : &map_k, 64 * d, 0, it.head, page, full);
+              }
+              __syncwarp();
+            }
+            page = next;
+          }
+        }
+      }
+    } else {
+      constexpr int kChunks = D / 16;         // 16-byte pieces of a key
+      constexpr int kKeys = 32 / kChunks;     // keys that the warp's lanes reach at once
+      const int w = warp - 8, key = w * 32 + lane;
+      const uint32_t raw = smem_u32(raw_s) + w * 32 * D;
+      for (int id = id0; id < n_items && ok && chunk_item(P, id, rank, cur, it); id += id_step) {
+        // this lane's key of step j: its page, or -1
+        auto page_of = [&](int j) -> int {
+          const int pos = ((it.lo + j) << 7) + key;
+          return j < it.steps && pos < it.n_keys ? kv_page(P.p, P.c, it.seq, pos) : -1;
+        };
+        auto fetch = [&](int j, int page, uint32_t stage, float &ks, float &vs) {
+          ks = vs = 0.f;
+          if (j < it.steps) {
+            const int slot = (((it.lo + j) << 7) + key) & ((1 << P.c.log2_page) - 1);
+            if (page >= 0) {
+              ks = __ldg(P.c.k.scale + page * P.c.k.scale_page + it.head * P.c.k.scale_head + slot);
+              vs = __ldg(P.c.v.scale + page * P.c.v.scale_page + it.head * P.c.v.scale_head + slot);
+            }
+            const uint32_t dst = raw + stage * S::kRaw;
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i) {
+              const int kk = i * kKeys + lane / kChunks, part = lane % kChunks;
+              const int pg = __shfl_sync(0xffffffffu, page, kk), sl = __shfl_sync(0xffffffffu, slot, kk);
+              const bool there = pg >= 0;
+              const int64_t at = there ? pg : 0;
+              chunk_copy16(dst + kk * D + part * 16, P.c.k.base + at * P.c.k.page + it.head * P.c.k.head + sl * P.c.k.slot + part * 16, there);
+              chunk_copy16(dst + 128 * D + kk * D + part * 16, P.c.v.base + at * P.c.v.page + it.head * P.c.v.head + sl * P.c.v.slot + part * 16, there);
+            }
+          }
+          asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        // widens the warp's 32 keys of a raw tile into the swizzled 16-bit tile
+        auto widen = [&](uint32_t src, uint32_t dst) {
+#pragma unroll
+          for (int i = 0; i < kChunks; ++i) {
+            const int kk = i * kKeys + lane / kChunks, part = lane % kChunks, row = w * 32 + kk;
+            uint32_t x[4], y[8];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(src + kk * D + part * 16) : "memory");
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              y[2 * e] = paged_widen2<HALF>(x[e], 0);
+              y[2 * e + 1] = paged_widen2<HALF>(x[e], 1);
+            }
+            const uint32_t base = dst + (part >> 2) * 16384 + row * 128, u = 2 * (part & 3);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + ((u ^ (row & 7)) << 4)), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + (((u + 1) ^ (row & 7)) << 4)), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7]) : "memory");
+          }
+        };
+        constexpr int kDeep = S::kRawStages;
+        float ks[kDeep], vs[kDeep];  // of the steps under way, the current one first
+#pragma unroll
+        for (int i = 0; i < kDeep - 1; ++i) fetch(i, page_of(i), (g + i) % kDeep, ks[i], vs[i]);
+        int page = page_of(kDeep - 1);
+        for (int j = 0; j < it.steps && ok; ++j, ++g) {
+          fetch(j + kDeep - 1, page, (g + kDeep - 1) % kDeep, ks[kDeep - 1], vs[kDeep - 1]);
+          page = page_of(j + kDeep);
+          asm volatile("cp.async.wait_group %0;" ::"n"(kDeep - 1) : "memory");
+          __syncwarp();
+          const uint32_t src = raw + (g % kDeep) * S::kRaw;
+          const uint32_t st = g % S::kStages, ph = ((g / S::kStages) & 1) ^ 1, slot = g % kScaleSlots;
+          if (!(ok = wait(&k_empty[st], ph, 33))) break;
+          widen(src, smem_u32(k_s) + st * S::kKV);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&k_full[st]);
+          if (!(ok = wait(&sc_empty[slot], ((g / kScaleSlots) & 1) ^ 1, 40))) break;
+          float *sc = scale_s + slot * (2 * 128 + 4);
+          sc[key] = ks[0];
+          sc[128 + key] = vs[0];
+          float top = fabsf(vs[0]);
+#pragma unroll
+          for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+          if (lane == 0) sc[256 + w] = top;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc_full[slot]);
+          if (!(ok = wait(&v_empty[st], ph, 33))) break;
+          widen(src + 128 * D, smem_u32(v_s) + st * S::kKV);
+          fence_proxy_async();
+          __syncwarp();  // every lane has read its raw bytes: the next fetch may overwrite them
+          if (lane == 0) mbar_arrive(&v_full[st]);
+#pragma unroll
+          for (int i = 0; i + 1 < kDeep; ++i) { ks[i] = ks[i + 1]; vs[i] = vs[i + 1]; }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    // ---- softmax ------------------------------------------------------------------------------------------------------
+    const int h = warp >> 2, tid = threadIdx.x & 127, row = h * 128 + tid;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + h * 128, o_addr = tmem + lanes + 256 + h * D;
+    const uint32_t p_addr = tmem + lanes + (S::kAhead ? 384 + h * 64 : h * 128);
+    const float c = P.a.c;
+    const float2 c2 = make_float2(c, c);
+    uint32_t g = 0, n = 0;
+    bool ok = true;
+    ChunkCursor cur;
+    ChunkItem it;
+    for (int id = id0; id < n_items && chunk_item(P, id, rank, cur, it); id += id_step) {
+      // last key that this row sees, and the warp's first row; rows that do not exist see what the last one does
+      const int lim = last_seen(it, row);
+      const int warp_lim = __shfl_sync(0xffffffffu, lim, 0);
+      float m = -INFINITY, l = 0.f, lv = 0.f;  // reference of the exponents: m * c + lv, lv = log2 of the value scales' power of two
+      bool have_lv = false;
+      auto absent_of = [&](int j) -> uint32_t {  // a bit for each 16 keys of step j that have no page
+        const int pos = ((it.lo + j) << 7) + 16 * (lane & 7);
+        return __ballot_sync(0xffffffffu, j < it.steps && pos < it.n_keys && kv_page(P.p, P.c, it.seq, pos) < 0) & 0xffu;
+      };
+      uint32_t absent = absent_of(0);
+      for (int j = 0; j < it.steps; ++j, ++g) {
+        const uint32_t absent_now = absent;
+        absent = absent_of(j + 1);
+        const uint32_t slot = g % kScaleSlots;
+        if (j >= it.blocks[h]) {
+          if (I8) {  // not before the slot is filled: a half that has nothing to do must not get ahead of the other
+            if (ok) ok = wait(&sc_full[slot], (g / kScaleSlots) & 1, 42);
+            if (ok && lane == 0) mbar_arrive(&sc_empty[slot]);
+          }
+          continue;
+        }
+        if (ok) ok = wait(&s_full[h], n & 1, 41);
+        if (I8 && ok) ok = wait(&sc_full[slot], (g / kScaleSlots) & 1, 42);
+        if (!ok) continue;
+        tc_fence_after();
+        uint32_t sa[4][32];
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) tmem_ld32_issue(s_addr + q4 * 32, sa[q4]);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (S::kAhead && lane == 0) mbar_arrive(&s_free[h]);
+        float s[128];
+#pragma unroll
+        for (int i = 0; i < 128; ++i) s[i] = __uint_as_float(sa[i >> 5][i & 31]);
+        const int key0 = (it.lo + j) << 7;
+        const float *sc = scale_s + slot * (2 * 128 + 4);
+        if (I8) {
+#pragma unroll
+          for (int i = 0; i < 128; i += 4) {
+            const float4 k4 = *reinterpret_cast<const float4 *>(sc + i);
+            const float2 x = mul2(make_float2(s[i], s[i + 1]), make_float2(k4.x, k4.y)), y = mul2(make_float2(s[i + 2], s[i + 3]), make_float2(k4.z, k4.w));
+            s[i] = x.x; s[i + 1] = x.y; s[i + 2] = y.x; s[i + 3] = y.y;
+          }
+        }
+        const bool masked = key0 + 127 > warp_lim || absent_now != 0;  // warp-uniform
+        const int last = lim - key0;  // last of the 128 that the row sees
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (i > last || ((absent_now >> (i >> 4)) & 1)) s[i] = -INFINITY;
+        }
+        float mq[8];
+#pragma unroll
+        for (int q8 = 0; q8 < 8; ++q8) {
+          mq[q8] = max3(s[16 * q8], s[16 * q8 + 1], s[16 * q8 + 2]);
+#pragma unroll
+          for (int i = 3; i + 1 < 16; i += 2) mq[q8] = max3(mq[q8], s[16 * q8 + i], s[16 * q8 + i + 1]);
+          mq[q8] = fmaxf(mq[q8], s[16 * q8 + 15]);
+        }
+        const float mx = fmaxf(max3(mq[0], mq[1], mq[2]), max3(max3(mq[3], mq[4], mq[5]), mq[6], mq[7]));
+        const float m_cand = fmaxf(m, mx);
+        const bool grow = (m_cand - m) * c > kChunkLazy;  // -inf -> finite: true; -inf -> -inf is NaN: false
+        const float m_new = grow ? m_cand : m;
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        float shift = grow ? (m - m_use) * c : 0.f;
+        if constexpr (I8 && HALF) {
+          // probabilities times value scales stay within fp16: the largest scale's power of two joins the reference
+          const float4 t4 = *reinterpret_cast<const float4 *>(sc + 256);
+          const uint32_t e = __float_as_uint(fmaxf(fmaxf(t4.x, t4.y), fmaxf(t4.z, t4.w))) >> 23;
+          const float lv_blk = (float)(int)e - 127.f;
+          if (e > 0 && e < 255 && (!have_lv || lv_blk > lv)) {
+            shift += have_lv ? lv - lv_blk : 0.f;
+            lv = lv_blk;
+            have_lv = true;
+          }
+        }
+        const float alpha = shift == 0.f ? 1.f : ex2f(shift);
+        const float nmc = -m_use * c - lv;
+        const float2 nmc2 = make_float2(nmc, nmc);
+        m = m_new;
+        if (n > 0) {
+          // the product before must have read P and updated O
+          ok = wait(&pv_done[h], (n - 1) & 1, 43);
+          if (!ok) continue;
+          tc_fence_after();
+          if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+#pragma unroll
+            for (int q4 = 0; q4 < D / 16; ++q4) {
+              uint32_t o[16];
+              tmem_ld16_issue(o_addr + q4 * 16, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st16(o_addr + q4 * 16, o);
+            }
+            tmem_st_wait();
+          }
+        }
+        float2 sq[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int i = 0; i < 64; i += 2) {
+            const int at = 64 * half + i;
+            const float2 e = fma2(make_float2(s[at], s[at + 1]), c2, nmc2);
+            // a quarter of the exponentials on the FMA pipe, as in attention_sm100.cu
+            float2 pp = ((i >> 1) & 3) == 3 ? ex2_fma2(e) : make_float2(ex2f(e.x), ex2f(e.y));
+            if (((i >> 1) & 3) == 3 && masked) {  // the polynomial's smallest value is not zero
+              if (s[at] == -INFINITY) pp.x = 0.f;
+              if (s[at + 1] == -INFINITY) pp.y = 0.f;
+            }
+            sq[(i >> 1) & 3] = add2(sq[(i >> 1) & 3], pp);
+            if (I8) {
+              const float2 v2 = *reinterpret_cast<const float2 *>(sc + 128 + at);
+              float2 t = mul2(pp, v2);
+              if (masked) {  // a token that is not seen may have a scale that is no number
+                if (s[at] == -INFINITY) t.x = 0.f;
+                if (s[at + 1] == -INFINITY) t.y = 0.f;
+              }
+              pp = t;
+            }
+            pk[i >> 1] = out_pair<HALF>(pp.x, pp.y);
+          }
+          tmem_st32(p_addr + half * 32, pk);
+        }
+        const float2 s01 = add2(sq[0], sq[1]), s23 = add2(sq[2], sq[3]);
+        l = l * alpha + ((s01.x + s01.y) + (s23.x + s23.y));
+        if (I8) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc_empty[slot]);
+        }
+        if (!I8 && (key0 + 127 > it.first_seen)) {
+          // This block's values: thread = key. What lies behind the context is zeroed, what only some rows see is made finite.
+          const uint32_t st = g % S::kStages;
+          ok = wait(&v_full[st], (g / S::kStages) & 1, 44);
+          if (!ok) continue;
+          const int key = key0 + tid;
+          uint8_t *vrow = v_s + st * S::kKV + tid * 128;
+          if (key > it.first_seen) {
+#pragma unroll
+            for (int u = 0; u < D / 8; ++u) {
+              uint4 *at = reinterpret_cast<uint4 *>(vrow + (u >> 3) * 16384 + (u & 7) * 16);  // the order in the row does not matter
+              if (key >= it.n_keys) {
+                *at = make_uint4(0, 0, 0, 0);
+              } else {
+                uint4 x = *at;
+                uint32_t *x4 = reinterpret_cast<uint32_t *>(&x);
+                bool hit = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) hit |= not_finite2<HALF>(x4[e]);
+                if (hit) {
+                  *poison = 1;
+                  __threadfence_block();
+                  for (int e = 0; e < 4; ++e) {
+                    if (not_finite2<HALF>(x4[e] & 0xffffu)) x4[e] &= 0xffff0000u;
+                    if (not_finite2<HALF>(x4[e] & 0xffff0000u)) x4[e] &= 0xffffu;
+                  }
+                  *at = x;
+                }
+              }
+            }
+          }
+          __threadfence_block();
+          fence_proxy_async();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[h]);
+        ++n;
+      }
+      // ---- the item's rows ----
+      if (!ok) continue;
+      const bool any = it.blocks[h] > 0;
+      if (any) {
+        ok = wait(&pv_done[h], (n - 1) & 1, 45);
+        if (!ok) continue;
+        tc_fence_after();
+      }
+      const bool seen = any && m != -INFINITY;  // the row met a key
+      if (P.splits > 1) {  // joined below
+        ml_s[row] = seen ? m * c + lv : -INFINITY;
+        ml_s[kChunkRows + row] = l;
+        continue;
+      }
+      const float inv = seen ? 1.0f / l : 0.f;
+      const bool slow = !I8 && any && *poison != 0;
+      uint8_t *out = out_row(it, row);
+#pragma unroll 1
+      for (int q4 = 0; q4 < D / 16; ++q4) {
+        float o[16];
+        load_o(it, o_addr, q4, any, seen, slow, lim, o);
+        if (row < it.rows) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = out_pair<HALF>(o[8 * i + 2 * k] * inv, o[8 * i + 2 * k + 1] * inv);
+            *reinterpret_cast<uint4 *>(out + q4 * 32 + i * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      tc_fence_before();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (P.splits == 1) {
+    if (warp == 12) tmem_dealloc(tmem, 512);
+    return;
+  }
+  // As many registers for everyone as at launch. Only behind the barrier: a role that is done early must not take back what
+  // the softmax warps have yet to receive.
+  if (run) {
+    if (warp < 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+  }
+
+  // ---- join the CTAs of the cluster ---------------------------------------------------------------------------------------
+  // Every role is done, so the rings are free: they take the partial rows, by columns of four, so that neighbouring rows fall
+  // into neighbouring banks.
+  tc_fence_after();
+  ChunkCursor cur;
+  ChunkItem it;
+  const bool good = run && *abort_flag == 0 && id0 < n_items && chunk_item(P, id0, rank, cur, it);
+  if (good && warp < 8) {
+    const int row = threadIdx.x, h = warp >> 2;
+    const bool any = it.blocks[h] > 0, seen = any && ml_s[row] != -INFINITY;
+    const uint32_t o_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 256 + h * D;
+    const int lim = last_seen(it, row);
+#pragma unroll 1
+    for (int q4 = 0; q4 < D / 16; ++q4) {
+      float o[16];
+      load_o(it, o_addr, q4, any, seen, !I8 && any && *poison != 0, lim, o);
+      float4 *st = reinterpret_cast<float4 *>(k_s) + q4 * 4 * kChunkRows + row;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) st[i * kChunkRows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+    }
+  }
+  tc_fence_before();
+  chunk_cluster_sync();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (good) {  // each CTA writes its share of the rows
+    constexpr int kParts = D / 8;  // eight values of a row per thread
+    const int r0 = kChunkRows * rank / P.splits, r1 = min(kChunkRows * (rank + 1) / P.splits, it.rows);
+    for (int i = (int)threadIdx.x + r0 * kParts; i < r1 * kParts; i += kChunkThreads) {
+      const int row = i / kParts, part = i % kParts;
+      float mm = -INFINITY;
+      for (int s = 0; s < P.splits; ++s) mm = fmaxf(mm, chunk_peer(smem_u32(ml_s + row), s));
+      float o[8] = {}, sum = 0.f;
+      if (mm != -INFINITY) {
+        for (int s = 0; s < P.splits; ++s) {
+          const float e = ex2f(chunk_peer(smem_u32(ml_s + row), s) - mm);
+          sum += chunk_peer(smem_u32(ml_s + kChunkRows + row), s) * e;
+          const uint32_t at = smem_u32(k_s) + ((part * 2) * kChunkRows + row) * 16;
+          const float4 x = chunk_peer4(at, s), y = chunk_peer4(at + kChunkRows * 16, s);
+          o[0] += x.x * e; o[1] += x.y * e; o[2] += x.z * e; o[3] += x.w * e;
+          o[4] += y.x * e; o[5] += y.y * e; o[6] += y.z * e; o[7] += y.w * e;
+        }
+      }
+      const float inv = mm != -INFINITY ? 1.0f / sum : 0.f;
+      *reinterpret_cast<uint4 *>(out_row(it, row) + part * 16) = make_uint4(out_pair<HALF>(o[0] * inv, o[1] * inv), out_pair<HALF>(o[2] * inv, o[3] * inv),
+                                                               out_pair<HALF>(o[4] * inv, o[5] * inv), out_pair<HALF>(o[6] * inv, o[7] * inv));
+    }
+  }
+  chunk_cluster_sync();  // nobody's shared memory goes away while it is read
+}
+
+template <bool HALF, int D, bool I8>
+static int launch(const ChunkParams &P, const CUtensorMap &mk, const CUtensorMap &mv, unsigned grid, cudaStream_t stream) {
+  using S = ChunkTile<D, I8>;
+  const auto kernel = paged_chunk_kernel<HALF, D, I8>;
+  // the attribute belongs to the device: set once on each, again where two threads meet
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    if (e != cudaSuccess) {
+      set_error(std::string("paged_attention: cannot raise the shared-memory limit: ") + cudaGetErrorString(e));
+      return PGB_ERR_CUDA;
+    }
+    if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kChunkThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = P.splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mk, mv, P);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_error(std::string("paged_chunk_kernel: ") + cudaGetErrorString(e));
+    return PGB_ERR_CUDA;
+  }
+  count_launch();
+  return PGB_OK;
+}
+
+// The pages as a 4-D tensor map: boxes of one page and 64 columns. False where TMA cannot address them.
+static bool page_map(CUtensorMap *m, const KvCache &c, const KvPages &p) {
+  const uint64_t P = (uint64_t)1 << c.log2_page;
+  const uint64_t dims[4] = {(uint64_t)c.head_dim, P, (uint64_t)c.heads, (uint64_t)c.n_pages};
+  // a dim of extent 1 still needs a valid stride
+  const uint64_t slot = (uint64_t)p.slot;
+  const uint64_t head = c.heads > 1 ? (uint64_t)p.head : slot * P;
+  const uint64_t page = c.n_pages > 1 ? (uint64_t)p.page : head * c.heads;
+  const uint64_t strides[3] = {slot, head, page};
+  const uint32_t box[4] = {64, (uint32_t)P, 1, 1};
+  for (uint64_t s : strides)
+    if (s == 0 || s >= (1ull << 40)) return false;
+  return encode_map_4d(m, c.dtype == PGB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.base, dims, strides, box);
+}
+
+bool run_paged_chunk(const PagedParams &a, const KvCache &c, const KvPlan &p, bool half, cudaStream_t stream, int *status) {
+  ChunkParams P{};
+  P.a = a;
+  P.c = c;
+  P.p = p;
+  // tiles of 256 rows: each sequence that has rows adds at most one that is not full
+  const int64_t k = std::min<int64_t>(p.n_seq, a.rows), tiles = (a.rows * a.group - k) / kChunkRows + k;
+  if (tiles * c.heads > 1073741824LL || c.n_pages == 0) return false;
+  CUtensorMap mk{}, mv{};
+  if (c.dtype != PGB_I8 && (!page_map(&mk, c, c.k) || !page_map(&mv, c, c.v))) return false;
+  P.n_tiles = (int)tiles;
+  const int64_t items = tiles * c.heads, blocks = ((int64_t)p.width << c.log2_page) / 128;
+  P.splits = 1;
+  while (P.splits < 8 && items * P.splits * 2 <= sm_count() && blocks >= 4LL * P.splits) P.splits *= 2;
+  P.err = gemm_error_word();
+  if (!P.err) {
+    set_error("paged_attention: cannot resolve the device error word");
+    *status = PGB_ERR_CUDA;
+    return true;
+  }
+  uint32_t drill_polls = 0;
+  take_next_wait_test(&drill_polls, &P.skip_loads);
+  P.polls = drill_polls ? drill_polls : kChunkPolls;
+  const unsigned grid = P.splits > 1 ? (unsigned)(items * P.splits) : (unsigned)std::min<int64_t>(items, sm_count());
+  const bool i8 = c.dtype == PGB_I8;
+#define PGB_CHUNK(H, D, Q) launch<H, D, Q>(P, mk, mv, grid, stream)
+  if (half) {
+    if (c.head_dim == 64) *status = i8 ? PGB_CHUNK(true, 64, true) : PGB_CHUNK(true, 64, false);
+    else *status = i8 ? PGB_CHUNK(true, 128, true) : PGB_CHUNK(true, 128, false);
+  } else {
+    if (c.head_dim == 64) *status = i8 ? PGB_CHUNK(false, 64, true) : PGB_CHUNK(false, 64, false);
+    else *status = i8 ? PGB_CHUNK(false, 128, true) : PGB_CHUNK(false, 128, false);
+  }
+#undef PGB_CHUNK
+  return true;
+}
+
+}  // namespace pgb

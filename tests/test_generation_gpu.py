@@ -183,6 +183,18 @@ def test_attention(new, ctx, dtype, cache, D, P, Hq, Hkv, layout):
     assert (out[plan.starts[-1]:] == 7).all()  # rows behind the last sequence
 
 
+@pytest.mark.parametrize("dtype,cache,D,P,Hq,Hkv", [(F16, F16, 64, 16, 12, 12), (F16, I8, 64, 32, 12, 12), (BF16, I8, 128, 64, 20, 20), (BF16, BF16, 128, 128, 20, 20)])
+@pytest.mark.parametrize("new,ctx", [([100, 90], [3000, 5000]), ([300, 64, 129], [4000, 4100, 2000]), ([90] * 20, [2000] * 20)])
+def test_halves_of_a_tile_that_end_apart(new, ctx, dtype, cache, D, P, Hq, Hkv):
+    # tiles whose second half is empty, short or a block longer, over many blocks of keys, several times in a row
+    plan = Plan(new, ctx, P)
+    c = new_cache(plan, Hkv, D, cache)
+    q = randn(plan.rows, Hq, D, dtype=dtype)
+    outs = [attend(plan, q, c) for _ in range(3)]
+    check(plan, outs[0], q, c)
+    assert same(outs[0], outs[1]) and same(outs[0], outs[2])
+
+
 @pytest.mark.parametrize("cache", [F16, I8])
 @pytest.mark.parametrize("new", [1, 3, 150])
 def test_scores_that_grow_and_shrink(new, cache):
