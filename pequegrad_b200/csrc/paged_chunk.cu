@@ -11,8 +11,8 @@
 //   warps 8-11      keys and values. 16 bits: one warp issues a TMA box per page (an index that is no page reads as zeros).
 //                   int8: each warp brings 32 keys a block into a raw ring with cp.async, widens them exactly to 16 bits and
 //                   stores them as the tiles TMA would have written; scales go to the softmax warps through a small ring.
-//   warp 12         tensor memory; issues the MMAs (one lane)
-//   warps 13-15     Q rows, by cp.async into the swizzled tiles
+//   warps 12, 13    issue the MMAs of A and of B (one lane each), so that neither half waits for the other's softmax
+//   warps 14, 15    Q rows, by cp.async into the swizzled tiles
 // Tensor memory: S_A [0, 128), S_B [128, 256), O_A, O_B behind them. With head dim 64 there is room for P beside S, and the
 // scores of the next block are computed under the softmax of this one; with 128 P takes the place of S, and the two halves
 // keep the tensor pipe and the exponentials busy in turn.
@@ -29,6 +29,7 @@
 #include <atomic>
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 #include "attention_ptx.cuh"
 #include "paged.cuh"
@@ -74,7 +75,9 @@ struct ChunkItem {
   int n_keys;            // keys that the item's last row sees
   int first_seen;        // last key that the item's first row sees
   int lo;                // first block of this CTA
-  int steps, blocks[2];  // blocks of this CTA; of each half
+  int steps, n_a, n_b;   // blocks of this CTA; those of half A and of half B
+
+  __device__ __forceinline__ int blocks(int half) const { return half ? n_b : n_a; }
 };
 
 struct ChunkCursor {
@@ -125,8 +128,16 @@ __device__ __forceinline__ bool chunk_item(const ChunkParams &P, int id, int ran
     const int n_a = (keys(min(it.rows, 128) - 1) + 127) >> 7, n_all = (it.n_keys + 127) >> 7;
     it.lo = n_all * rank / P.splits;
     it.steps = n_all * (rank + 1) / P.splits - it.lo;
-    it.blocks[0] = max(0, min(it.steps, n_a - it.lo));
-    it.blocks[1] = it.rows > 128 ? it.steps : 0;
+    it.n_a = max(0, min(it.steps, n_a - it.lo));
+    it.n_b = it.rows > 128 ? it.steps : 0;
+    // every lane has the same values; a broadcast tells the compiler so
+    it.steps = __shfl_sync(0xffffffffu, it.steps, 0);
+    it.n_a = __shfl_sync(0xffffffffu, it.n_a, 0);
+    it.n_b = __shfl_sync(0xffffffffu, it.n_b, 0);
+    it.lo = __shfl_sync(0xffffffffu, it.lo, 0);
+    it.seq = __shfl_sync(0xffffffffu, it.seq, 0);
+    it.first_seen = __shfl_sync(0xffffffffu, it.first_seen, 0);
+    it.n_keys = __shfl_sync(0xffffffffu, it.n_keys, 0);
     return true;
   }
   return false;
@@ -160,6 +171,14 @@ __device__ __forceinline__ float4 chunk_peer4(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void chunk_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Waits for this thread's loads from tensor memory and ties their registers to the wait.
+__device__ __forceinline__ void chunk_ld_wait(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
+                 "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]),
+                 "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]),
+                 "+r"(v[31])::"memory");
 }
 // exponent all ones in either half of a word of two 16-bit floats
 template <bool HALF>
@@ -197,20 +216,21 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
   int *dead = const_cast<int *>(abort_flag) + 1;
   volatile int *poison = const_cast<volatile int *>(abort_flag) + 2;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // broadcast, so that the compiler knows it is the same for the warp: barrier addresses and descriptors stay uniform
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = P.splits > 1 ? (int)(blockIdx.x % P.splits) : 0;
   const int n_items = P.n_tiles * P.c.heads;
   // one item per cluster, or every gridDim.x-th
   const int id0 = (int)blockIdx.x / P.splits, id_step = P.splits > 1 ? n_items : (int)gridDim.x;
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 3);
-    mbar_init(q_empty, 1);
+    mbar_init(q_full, 2);
+    mbar_init(q_empty, 2);
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(&k_full[s], I8 ? 4 : 1);
       mbar_init(&v_full[s], I8 ? 4 : 1);
-      mbar_init(&k_empty[s], 1);
-      mbar_init(&v_empty[s], 1);
+      mbar_init(&k_empty[s], 2);  // the MMAs of A and of B
+      mbar_init(&v_empty[s], 2);
     }
     for (int s = 0; s < kScaleSlots; ++s) {
       mbar_init(&sc_full[s], 4);
@@ -278,12 +298,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     }
     return ok;
   };
-  // 128 launch registers a thread are dealt out anew: 184 + 184 + 64 + 80 = 4 * 128
   if (!run) {
   } else if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp > 12) {
-    // ---- Q: 96 lanes, 16-byte pieces; rows that do not exist are zeros --------------------------------------------
+    if (warp > 13) {
+    // ---- Q: 64 lanes, 16-byte pieces; rows that do not exist are zeros --------------------------------------------
     ChunkCursor cur;
     ChunkItem it;
     uint32_t n = 0;
@@ -292,7 +310,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       if (!wait(q_empty, (n & 1) ^ 1, 32)) break;
       ++n;
       constexpr int kUnits = D / 8;
-      for (int i = (warp - 13) * 32 + lane; i < kChunkRows * kUnits; i += 96) {
+      for (int i = (warp - 14) * 32 + lane; i < kChunkRows * kUnits; i += 64) {
         const int r = i / kUnits, u = i % kUnits;
         const bool in = r < it.rows;
         const int pr = it.sub + (in ? r : 0), tok = pr / P.a.group, g = pr - tok * P.a.group;
@@ -307,51 +325,57 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       if (lane == 0) mbar_arrive(q_full);
     }
     } else {
-    // ---- MMA ------------------------------------------------------------------------------------------------------
+    // ---- MMA of one half ----------------------------------------------------------------------------------------------
+    // A half that has nothing in a step still waits for the step's operands before it gives them up: its arrivals must not
+    // run ahead of the other half's.
+    const int h = warp - 12;
     const uint32_t idesc_s = attn_idesc(HALF, false, 128), idesc_pv = attn_idesc(HALF, true, D);
-    const uint32_t col_p[2] = {S::kAhead ? 384u : 0u, S::kAhead ? 448u : 128u}, col_o[2] = {256u, 256u + D};
+    const uint32_t t_s = tmem + h * 128, t_p = S::kAhead ? tmem + 384 + h * 64 : t_s, t_o = tmem + 256 + h * D;
+    const uint32_t q_at = smem_u32(q_s) + h * (S::kQ / 2);
     ChunkCursor s_cur, cur;
     ChunkItem s_it, it;
     int s_id = id0, s_j = 0;
     bool s_more = false;
     auto s_seek = [&]() {  // the next item with blocks for this CTA
+      s_more = false;
       for (; s_id < n_items; s_id += id_step) {
-        if (!chunk_item(P, s_id, rank, s_cur, s_it)) break;
+        if (!chunk_item(P, s_id, rank, s_cur, s_it)) return;
         if (s_it.steps > 0) { s_more = true; return; }
       }
-      s_more = false;
     };
     s_seek();
-    uint32_t s_g = 0, s_items = 0, s_n[2] = {0, 0};
-    // scores of half h in the step of the S cursor
-    auto issue_s = [&](int h) -> bool {
-      if (s_j >= s_it.blocks[h]) return true;
-      const uint32_t ks = s_g % S::kStages;
-      if (S::kAhead && !wait(&s_free[h], (s_n[h] & 1) ^ 1, 36)) return false;
-      tc_fence_after();
-      if (lane == 0) {
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * 16384;
-          tc_mma<kKind>(tmem + h * 128, make_kmajor_sw128_desc(smem_u32(q_s) + h * (S::kQ / 2) + off) + 2 * (kk & 3),
-                        make_kmajor_sw128_desc(smem_u32(k_s) + ks * S::kKV + off) + 2 * (kk & 3), idesc_s, kk != 0);
-        }
-        tc_commit(&s_full[h]);
-      }
-      __syncwarp();
-      ++s_n[h];
-      return true;
-    };
-    auto s_operands = [&]() -> bool {
+    uint32_t s_g = 0, s_items = 0, s_n = 0, g = 0, n = 0;
+    // scores of the step at the S cursor, one step ahead of the products
+    auto issue_s = [&]() -> bool {
       if (s_j == 0 && !wait(q_full, s_items & 1, 34)) return false;
-      return wait(&k_full[s_g % S::kStages], (s_g / S::kStages) & 1, 35);
-    };
-    auto s_next = [&]() {
+      const uint32_t ks = s_g % S::kStages;
+      if (!wait(&k_full[ks], (s_g / S::kStages) & 1, 35)) return false;
+      const bool active = s_j < s_it.blocks(h), last = s_j + 1 == s_it.steps;
+      if (active) {
+        if (S::kAhead) {
+          if (!wait(&s_free[h], (s_n & 1) ^ 1, 36)) return false;
+        } else if (n > 0 && !wait(&pv_done[h], (n - 1) & 1, 39)) {  // P lies where these scores go
+          return false;
+        }
+        tc_fence_after();
+      }
       if (lane == 0) {
-        tc_commit(&k_empty[s_g % S::kStages]);
-        if (s_j + 1 == s_it.steps) tc_commit(q_empty);
+        if (active) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * 16384;
+            tc_mma<kKind>(t_s, make_kmajor_sw128_desc(q_at + off) + 2 * (kk & 3), make_kmajor_sw128_desc(smem_u32(k_s) + ks * S::kKV + off) + 2 * (kk & 3), idesc_s, kk != 0);
+          }
+          tc_commit(&s_full[h]);
+          tc_commit(&k_empty[ks]);
+          if (last) tc_commit(q_empty);
+        } else {
+          mbar_arrive(&k_empty[ks]);
+          if (last) tc_commit(q_empty);  // behind this half's earlier products
+        }
       }
       __syncwarp();
+      s_n += active;
       ++s_g;
       if (++s_j == s_it.steps) {
         ++s_items;
@@ -359,57 +383,35 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         s_id += id_step;
         s_seek();
       }
+      return true;
     };
-    bool ok = true;
-    if (s_more) {
-      ok = s_operands() && issue_s(0) && issue_s(1);
-      if (ok) s_next();
-    }
-    uint32_t g = 0, n[2] = {0, 0};
+    bool ok = !s_more || issue_s();
     for (int id = id0; id < n_items && ok && chunk_item(P, id, rank, cur, it); id += id_step) {
       for (int j = 0; j < it.steps && ok; ++j, ++g) {
-        const uint32_t vs = g % S::kStages;
-        auto issue_pv = [&](int h) -> bool {
-          if (j >= it.blocks[h]) return true;
-          if (!wait(&p_full[h], n[h] & 1, 37)) return false;
-          if (!wait(&v_full[vs], (g / S::kStages) & 1, 38)) return false;
-          tc_fence_after();
-          if (lane == 0) {
+        if (S::kAhead && s_more && !(ok = issue_s())) break;
+        const uint32_t vs = g % S::kStages, ph = (g / S::kStages) & 1;
+        const bool active = j < it.blocks(h);
+        if (active && !(ok = wait(&p_full[h], n & 1, 37))) break;
+        if (!(ok = wait(&v_full[vs], ph, 38))) break;
+        tc_fence_after();
+        if (lane == 0) {
+          if (active) {
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)  // 16 keys per MMA: 8 columns of P, 16 rows of V
-              tc_mma_ts(tmem + col_o[h], tmem + col_p[h] + kk * 8, make_mnmajor_sw128_desc(smem_u32(v_s) + vs * S::kKV + kk * 2048, 16384), idesc_pv, (j | kk) != 0);
+              tc_mma_ts(t_o, t_p + kk * 8, make_mnmajor_sw128_desc(smem_u32(v_s) + vs * S::kKV + kk * 2048, 16384), idesc_pv, (j | kk) != 0);
             tc_commit(&pv_done[h]);
+            tc_commit(&v_empty[vs]);
+          } else {
+            mbar_arrive(&v_empty[vs]);
           }
-          __syncwarp();
-          ++n[h];
-          return true;
-        };
-        if (S::kAhead) {
-          if (s_more) {
-            ok = s_operands() && issue_s(0) && issue_s(1);
-            if (ok) s_next();
-          }
-          ok = ok && issue_pv(0) && issue_pv(1);
-        } else {
-          // P lies where the next scores go: they wait for the product that reads it
-          const bool more = s_more;
-          for (int h = 0; h < 2 && ok; ++h) {
-            ok = issue_pv(h);
-            if (ok && more) {
-              if (h == 0) ok = s_operands();
-              if (ok && n[h] > 0) ok = wait(&pv_done[h], (n[h] - 1) & 1, 39);
-              ok = ok && issue_s(h);
-            }
-          }
-          if (ok && more) s_next();
         }
-        if (ok && lane == 0) tc_commit(&v_empty[vs]);
         __syncwarp();
+        n += active;
+        if (!S::kAhead && s_more) ok = issue_s();
       }
     }
     }
   } else if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     // ---- keys and values --------------------------------------------------------------------------------------------
     ChunkCursor cur;
     ChunkItem it;
@@ -535,7 +537,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     // ---- softmax ------------------------------------------------------------------------------------------------------
     const int h = warp >> 2, tid = threadIdx.x & 127, row = h * 128 + tid;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -553,16 +554,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       const int warp_lim = __shfl_sync(0xffffffffu, lim, 0);
       float m = -INFINITY, l = 0.f, lv = 0.f;  // reference of the exponents: m * c + lv, lv = log2 of the value scales' power of two
       bool have_lv = false;
-      auto absent_of = [&](int j) -> uint32_t {  // a bit for each 16 keys of step j that have no page
-        const int pos = ((it.lo + j) << 7) + 16 * (lane & 7);
-        return __ballot_sync(0xffffffffu, j < it.steps && pos < it.n_keys && kv_page(P.p, P.c, it.seq, pos) < 0) & 0xffu;
+      auto page_of = [&](int j) -> int {  // of this lane's sixteen keys of step j; looked up a step early, used when it is there
+        const int i = (((it.lo + j) << 7) + 16 * (lane & 7)) >> P.c.log2_page;
+        return j < it.steps && (i << P.c.log2_page) < it.n_keys ? __ldg(P.p.table + (int64_t)it.seq * P.p.pitch + i) : 0;
       };
-      uint32_t absent = absent_of(0);
+      int page_next = page_of(0);
       for (int j = 0; j < it.steps; ++j, ++g) {
-        const uint32_t absent_now = absent;
-        absent = absent_of(j + 1);
+        const int page_now = page_next;
+        page_next = page_of(j + 1);
         const uint32_t slot = g % kScaleSlots;
-        if (j >= it.blocks[h]) {
+        if (j >= it.blocks(h)) {
           if (I8) {  // not before the slot is filled: a half that has nothing to do must not get ahead of the other
             if (ok) ok = wait(&sc_full[slot], (g / kScaleSlots) & 1, 42);
             if (ok && lane == 0) mbar_arrive(&sc_empty[slot]);
@@ -573,42 +574,57 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         if (I8 && ok) ok = wait(&sc_full[slot], (g / kScaleSlots) & 1, 42);
         if (!ok) continue;
         tc_fence_after();
-        uint32_t sa[4][32];
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) tmem_ld32_issue(s_addr + q4 * 32, sa[q4]);
-        tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (S::kAhead && lane == 0) mbar_arrive(&s_free[h]);
-        float s[128];
-#pragma unroll
-        for (int i = 0; i < 128; ++i) s[i] = __uint_as_float(sa[i >> 5][i & 31]);
+        // Two passes over the row of S, 32 columns at a time, the next 32 on their way: the maximum, then the probabilities.
+        // Reading tensor memory twice is cheaper than holding 128 scores: the loop's code stays in the instruction cache
+        // and its registers leave room.
+        uint32_t x0[32], x1[32];
+        tmem_ld32_issue(s_addr, x0);
+        const uint32_t absent = __ballot_sync(0xffffffffu, (unsigned)page_now >= (unsigned)P.c.n_pages) & 0xffu;  // a bit for each 16 keys without a page
         const int key0 = (it.lo + j) << 7;
+        const bool masked = key0 + 127 > warp_lim || absent != 0;  // warp-uniform
+        const int last = lim - key0;                               // last of the 128 that the row sees
         const float *sc = scale_s + slot * (2 * 128 + 4);
-        if (I8) {
+        float mx = -INFINITY;
+        // The first pass scales int8 scores by their keys and puts -inf where the row must not look; it writes what it changed
+        // back, so that the second pass takes every score as it finds it.
+        auto top = [&](uint32_t (&x)[32], int c) {
+          if (I8) {
 #pragma unroll
-          for (int i = 0; i < 128; i += 4) {
-            const float4 k4 = *reinterpret_cast<const float4 *>(sc + i);
-            const float2 x = mul2(make_float2(s[i], s[i + 1]), make_float2(k4.x, k4.y)), y = mul2(make_float2(s[i + 2], s[i + 3]), make_float2(k4.z, k4.w));
-            s[i] = x.x; s[i + 1] = x.y; s[i + 2] = y.x; s[i + 3] = y.y;
+            for (int i = 0; i < 32; i += 4) {
+              const float4 k4 = *reinterpret_cast<const float4 *>(sc + c + i);
+              const float2 u = mul2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), make_float2(k4.x, k4.y));
+              const float2 v = mul2(make_float2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), make_float2(k4.z, k4.w));
+              x[i] = __float_as_uint(u.x); x[i + 1] = __float_as_uint(u.y); x[i + 2] = __float_as_uint(v.x); x[i + 3] = __float_as_uint(v.y);
+            }
           }
-        }
-        const bool masked = key0 + 127 > warp_lim || absent_now != 0;  // warp-uniform
-        const int last = lim - key0;  // last of the 128 that the row sees
-        if (masked) {
+          if (masked) {
+            const uint32_t gone = absent >> (c >> 4);
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i > last || ((absent_now >> (i >> 4)) & 1)) s[i] = -INFINITY;
-        }
-        float mq[8];
+            for (int i = 0; i < 32; ++i)
+              if (c + i > last || ((gone >> (i >> 4)) & 1)) x[i] = 0xff800000u;  // -inf
+          }
+          if (I8 || masked) tmem_st32(s_addr + c, x);
+          float mq[4];
 #pragma unroll
-        for (int q8 = 0; q8 < 8; ++q8) {
-          mq[q8] = max3(s[16 * q8], s[16 * q8 + 1], s[16 * q8 + 2]);
-#pragma unroll
-          for (int i = 3; i + 1 < 16; i += 2) mq[q8] = max3(mq[q8], s[16 * q8 + i], s[16 * q8 + i + 1]);
-          mq[q8] = fmaxf(mq[q8], s[16 * q8 + 15]);
+          for (int q = 0; q < 4; ++q) {
+            mq[q] = max3(__uint_as_float(x[8 * q]), __uint_as_float(x[8 * q + 1]), __uint_as_float(x[8 * q + 2]));
+            mq[q] = max3(mq[q], __uint_as_float(x[8 * q + 3]), __uint_as_float(x[8 * q + 4]));
+            mq[q] = max3(mq[q], __uint_as_float(x[8 * q + 5]), __uint_as_float(x[8 * q + 6]));
+            mq[q] = fmaxf(mq[q], __uint_as_float(x[8 * q + 7]));
+          }
+          mx = max3(mx, max3(mq[0], mq[1], mq[2]), mq[3]);
+        };
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 64) {
+          chunk_ld_wait(x0);
+          tmem_ld32_issue(s_addr + c + 32, x1);
+          top(x0, c);
+          chunk_ld_wait(x1);
+          if (c == 0) tmem_ld32_issue(s_addr + 64, x0);
+          top(x1, c + 32);
         }
-        const float mx = fmaxf(max3(mq[0], mq[1], mq[2]), max3(max3(mq[3], mq[4], mq[5]), mq[6], mq[7]));
+        if (I8 || masked) tmem_st_wait();
+        tmem_ld32_issue(s_addr, x0);
         const float m_cand = fmaxf(m, mx);
         const bool grow = (m_cand - m) * c > kChunkLazy;  // -inf -> finite: true; -inf -> -inf is NaN: false
         const float m_new = grow ? m_cand : m;
@@ -648,32 +664,49 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
           }
         }
         float2 sq[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        auto exps = [&](uint32_t (&x)[32], int c) {
+          uint32_t pk[16];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int i = 0; i < 64; i += 2) {
-            const int at = 64 * half + i;
-            const float2 e = fma2(make_float2(s[at], s[at + 1]), c2, nmc2);
+          for (int i = 0; i < 32; i += 4) {
+            const float s[4] = {__uint_as_float(x[i]), __uint_as_float(x[i + 1]), __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])};
+            const float2 e0 = fma2(make_float2(s[0], s[1]), c2, nmc2), e1 = fma2(make_float2(s[2], s[3]), c2, nmc2);
+            float2 p0 = make_float2(ex2f(e0.x), ex2f(e0.y));
             // a quarter of the exponentials on the FMA pipe, as in attention_sm100.cu
-            float2 pp = ((i >> 1) & 3) == 3 ? ex2_fma2(e) : make_float2(ex2f(e.x), ex2f(e.y));
-            if (((i >> 1) & 3) == 3 && masked) {  // the polynomial's smallest value is not zero
-              if (s[at] == -INFINITY) pp.x = 0.f;
-              if (s[at + 1] == -INFINITY) pp.y = 0.f;
+            float2 p1 = (i & 4) ? ex2_fma2(e1) : make_float2(ex2f(e1.x), ex2f(e1.y));
+            if ((i & 4) && masked) {  // whose smallest value is not zero
+              p1.x = s[2] == -INFINITY ? 0.f : p1.x;
+              p1.y = s[3] == -INFINITY ? 0.f : p1.y;
             }
-            sq[(i >> 1) & 3] = add2(sq[(i >> 1) & 3], pp);
+            sq[(i >> 1) & 2] = add2(sq[(i >> 1) & 2], p0);
+            sq[((i >> 1) & 2) + 1] = add2(sq[((i >> 1) & 2) + 1], p1);
             if (I8) {
-              const float2 v2 = *reinterpret_cast<const float2 *>(sc + 128 + at);
-              float2 t = mul2(pp, v2);
+              const float4 v4 = *reinterpret_cast<const float4 *>(sc + 128 + c + i);
+              float2 t0 = mul2(p0, make_float2(v4.x, v4.y)), t1 = mul2(p1, make_float2(v4.z, v4.w));
               if (masked) {  // a token that is not seen may have a scale that is no number
-                if (s[at] == -INFINITY) t.x = 0.f;
-                if (s[at + 1] == -INFINITY) t.y = 0.f;
+                t0 = make_float2(p0.x == 0.f ? 0.f : t0.x, p0.y == 0.f ? 0.f : t0.y);
+                t1 = make_float2(p1.x == 0.f ? 0.f : t1.x, p1.y == 0.f ? 0.f : t1.y);
               }
-              pp = t;
+              p0 = t0;
+              p1 = t1;
             }
-            pk[i >> 1] = out_pair<HALF>(pp.x, pp.y);
+            pk[i >> 1] = out_pair<HALF>(p0.x, p0.y);
+            pk[(i >> 1) + 1] = out_pair<HALF>(p1.x, p1.y);
           }
-          tmem_st32(p_addr + half * 32, pk);
+          tmem_st16(p_addr + (c >> 1), pk);  // where P shares S's columns: those of scores already in registers
+        };
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 64) {
+          chunk_ld_wait(x0);
+          tmem_ld32_issue(s_addr + c + 32, x1);
+          exps(x0, c);
+          chunk_ld_wait(x1);
+          if (c == 0) tmem_ld32_issue(s_addr + 64, x0);
+          else if (S::kAhead) {  // every score is in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[h]);
+          }
+          exps(x1, c + 32);
         }
         const float2 s01 = add2(sq[0], sq[1]), s23 = add2(sq[2], sq[3]);
         l = l * alpha + ((s01.x + s01.y) + (s23.x + s23.y));
@@ -723,7 +756,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       }
       // ---- the item's rows ----
       if (!ok) continue;
-      const bool any = it.blocks[h] > 0;
+      const bool any = it.blocks(h) > 0;
       if (any) {
         ok = wait(&pv_done[h], (n - 1) & 1, 45);
         if (!ok) continue;
@@ -762,12 +795,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     if (warp == 12) tmem_dealloc(tmem, 512);
     return;
   }
-  // As many registers for everyone as at launch. Only behind the barrier: a role that is done early must not take back what
-  // the softmax warps have yet to receive.
-  if (run) {
-    if (warp < 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
-    else asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
-  }
 
   // ---- join the CTAs of the cluster ---------------------------------------------------------------------------------------
   // Every role is done, so the rings are free: they take the partial rows, by columns of four, so that neighbouring rows fall
@@ -778,7 +805,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
   const bool good = run && *abort_flag == 0 && id0 < n_items && chunk_item(P, id0, rank, cur, it);
   if (good && warp < 8) {
     const int row = threadIdx.x, h = warp >> 2;
-    const bool any = it.blocks[h] > 0, seen = any && ml_s[row] != -INFINITY;
+    const bool any = it.blocks(h) > 0, seen = any && ml_s[row] != -INFINITY;
     const uint32_t o_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 256 + h * D;
     const int lim = last_seen(it, row);
 #pragma unroll 1
