@@ -12,7 +12,9 @@
 //                   int8: each warp brings 32 keys a block into a raw ring with cp.async, widens them exactly to 16 bits and
 //                   stores them as the tiles TMA would have written; scales go to the softmax warps through a small ring.
 //   warps 12, 13    issue the MMAs of A and of B (one lane each), so that neither half waits for the other's softmax
-//   warps 14, 15    Q rows, by cp.async into the swizzled tiles
+//   warp 14         Q rows, by cp.async into the swizzled tiles (warps 9-11 help where keys come by TMA)
+//   warp 15         finds the items, some ahead of their use: the search's loads and divisions stay out of the other roles' way
+//                   and its code is there once
 // Tensor memory: S_A [0, 128), S_B [128, 256), O_A, O_B behind them. With head dim 64 there is room for P beside S, and the
 // scores of the next block are computed under the softmax of this one; with 128 P takes the place of S, and the two halves
 // keep the tensor pipe and the exponentials busy in turn.
@@ -41,6 +43,8 @@ constexpr int kChunkThreads = 512;
 constexpr uint32_t kChunkPolls = 1u << 20;
 constexpr float kChunkLazy = 8.0f;  // log2 of the largest probability before a row's reference moves
 constexpr int kScaleSlots = 4;
+constexpr int kItemSlots = 4;  // items found ahead
+constexpr int kItemReaders = 15;  // warps that read them: all but the one that finds them
 
 template <int D, bool I8>
 struct ChunkTile {
@@ -50,8 +54,8 @@ struct ChunkTile {
   static constexpr int kRawStages = I8 ? (D == 64 ? 3 : 2) : 0;
   static constexpr int kRing = 2 * kStages * kKV + kRawStages * kRaw;
   static constexpr int kScales = I8 ? kScaleSlots * (2 * 128 + 4) * 4 : 0;
-  static constexpr int kMl = 2 * kChunkRows * 4;
-  static constexpr int kSmem = kQ + kRing + kScales + kMl + 512 /*barriers*/ + 1024 /*alignment*/;
+  static constexpr int kMl = 3 * kChunkRows * 4;  // m and l of the rows, weights of the parts
+  static constexpr int kSmem = kQ + kRing + kScales + kMl + kItemSlots * 64 + 512 /*barriers*/ + 1024 /*alignment*/;
   static_assert(kRing >= kChunkRows * D * 4, "the partial results of a split item take the place of the rings");
   static_assert(kSmem <= 232448, "shared memory of one SM");
 };
@@ -80,27 +84,54 @@ struct ChunkItem {
   __device__ __forceinline__ int blocks(int half) const { return half ? n_b : n_a; }
 };
 
+// x / group; without grouped heads there is nothing to divide
+__device__ __forceinline__ int chunk_div(int x, int group) { return group == 1 ? x : (int)((unsigned)x / (unsigned)group); }
+
 struct ChunkCursor {
+  int hi = 0, lo = 0;  // tiles with keys in (lo, hi] are being dealt out; hi == 0: not begun
   int seq0 = 0, base = 0;
 };
 
-// Tile `t` of the list of all sequences' tiles, found by a warp: sequences 32 at a time. Tiles are asked for in ascending
-// order, so the search resumes where it stopped. False past the last tile.
+// Item `id` (tile id / heads, key head id % heads), found by a warp, sequences 32 at a time. The tiles are listed by the
+// number of keys that their last row sees, in bands of an eighth, most first: heavy items that start first even out. Within
+// a sequence that number grows with the tile, so how many of its tiles lie in a band takes no search. Items are asked for in
+// ascending order, so the search resumes where it stopped. False past the last tile.
 __device__ __forceinline__ bool chunk_item(const ChunkParams &P, int id, int rank, ChunkCursor &cur, ChunkItem &it) {
+  constexpr int kAll = -2147483647 - 1;
   const int lane = threadIdx.x & 31;
   const int t = id / P.c.heads;
   it.head = id - t * P.c.heads;
-  for (; cur.seq0 < P.p.n_seq; cur.seq0 += 32) {
+  if (cur.hi == 0) {
+    int most = 0;
+    for (int s = lane; s < P.p.n_seq; s += 32) most = max(most, __ldg(P.p.ctx + s));
+    most = __reduce_max_sync(0xffffffffu, most);
+    cur.hi = 2147483647;
+    cur.lo = most - (most >> 3);
+  }
+  for (;;) {
+    if (cur.seq0 >= P.p.n_seq) {
+      if (cur.lo == kAll) return false;
+      cur.hi = cur.lo;
+      cur.lo = cur.lo > 64 ? cur.lo - (cur.lo >> 3) : kAll;
+      cur.seq0 = 0;
+    }
     const int s = cur.seq0 + lane;
     int64_t start = 0, n = 0;
+    int ctx = 0;
     if (s < P.p.n_seq) {
       start = __ldg(P.p.start + s);
       n = min((int64_t)__ldg(P.p.start + s + 1), P.a.rows) - start;
+      ctx = __ldg(P.p.ctx + s);
       if (n < 0 || start < 0) n = 0;  // offsets that make no sense hold no rows
     }
-    const int64_t packed = n * P.a.group;
-    const int tiles = (int)((packed + kChunkRows - 1) / kChunkRows);
-    int sum = tiles;
+    const int tiles = (int)((n * P.a.group + kChunkRows - 1) / kChunkRows);
+    auto above = [&](int keys) -> int {  // tiles of this lane's sequence with more keys than that
+      if (keys == kAll) return tiles;
+      if (ctx <= keys) return 0;
+      return tiles - (int)min((int64_t)max(0, tiles - 1), max((int64_t)0, (keys - (ctx - n)) * P.a.group / kChunkRows));
+    };
+    const int top = above(cur.hi), count = above(cur.lo) - top;
+    int sum = count;
 #pragma unroll
     for (int k = 1; k < 32; k <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, sum, k);
@@ -109,20 +140,22 @@ __device__ __forceinline__ bool chunk_item(const ChunkParams &P, int id, int ran
     const uint32_t hit = __ballot_sync(0xffffffffu, t < cur.base + sum);
     if (!hit) {
       cur.base += __shfl_sync(0xffffffffu, sum, 31);
+      cur.seq0 += 32;
       continue;
     }
     const int src = __ffs(hit) - 1;
-    const int before = cur.base + __shfl_sync(0xffffffffu, sum - tiles, src);
+    const int tile = __shfl_sync(0xffffffffu, tiles - 1 - top - (t - cur.base - (sum - count)), src);
     n = __shfl_sync(0xffffffffu, n, src);
     it.seq = cur.seq0 + src;
     start = __shfl_sync(0xffffffffu, start, src);
-    const int64_t row0 = (int64_t)(t - before) * kChunkRows, tok0 = row0 / P.a.group;
+    const int64_t row0 = (int64_t)tile * kChunkRows;
+    const int64_t tok0 = row0 < 2147483647LL ? (int64_t)chunk_div((int)row0, P.a.group) : row0 / P.a.group;
     it.token = (int)(start + tok0);
     it.sub = (int)(row0 - tok0 * P.a.group);
     it.rows = (int)min((int64_t)kChunkRows, n * P.a.group - row0);
     const int held = P.p.width << P.c.log2_page;  // at most 2^30
     it.pos = (int)max(kv_position(P.p, it.seq, it.token), -((int64_t)1 << 31));
-    auto keys = [&](int row) { return max(0, min(held, it.pos + (it.sub + row) / P.a.group + 1)); };
+    auto keys = [&](int row) { return max(0, min(held, it.pos + chunk_div(it.sub + row, P.a.group) + 1)); };
     it.first_seen = keys(0) - 1;
     it.n_keys = keys(it.rows - 1);
     const int n_a = (keys(min(it.rows, 128) - 1) + 127) >> 7, n_all = (it.n_keys + 127) >> 7;
@@ -140,7 +173,6 @@ __device__ __forceinline__ bool chunk_item(const ChunkParams &P, int id, int ran
     it.n_keys = __shfl_sync(0xffffffffu, it.n_keys, 0);
     return true;
   }
-  return false;
 }
 
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -197,6 +229,7 @@ template <bool HALF, int D, bool I8>
 __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                        const __grid_constant__ ChunkParams P) {
   using S = ChunkTile<D, I8>;
+  constexpr int kQWarps = I8 ? 1 : 4;  // 14 and, where keys come by TMA, 9-11
   constexpr int kKind = GEMM_F16;  // kind::f16 serves both 16-bit types; the descriptor tells them apart
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -205,13 +238,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
   uint8_t *v_s = k_s + S::kStages * S::kKV;
   uint8_t *raw_s = v_s + S::kStages * S::kKV;   // [stage][K, V][128 keys][D bytes]
   float *scale_s = reinterpret_cast<float *>(raw_s + S::kRawStages * S::kRaw);  // [slot][128 of K, 128 of V, 4 maxima]
-  float *ml_s = scale_s + S::kScales / 4;       // [m, l][256]
-  uint64_t *bars = reinterpret_cast<uint64_t *>(ml_s + 2 * kChunkRows);
+  float *ml_s = scale_s + S::kScales / 4;       // [m, l][256], [part][rows that this CTA writes]
+  int4 *item_s = reinterpret_cast<int4 *>(ml_s + 3 * kChunkRows);  // [slot][4]
+  uint64_t *bars = reinterpret_cast<uint64_t *>(item_s + 4 * kItemSlots);
   uint64_t *q_full = bars, *q_empty = bars + 1;
   uint64_t *k_full = bars + 2, *k_empty = k_full + 4, *v_full = k_empty + 4, *v_empty = v_full + 4;  // [kStages]
   uint64_t *sc_full = v_empty + 4, *sc_empty = sc_full + kScaleSlots;
   uint64_t *s_full = sc_empty + kScaleSlots, *s_free = s_full + 2, *p_full = s_free + 2, *pv_done = p_full + 2;  // [half]
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(pv_done + 2);
+  uint64_t *item_full = pv_done + 2, *item_empty = item_full + kItemSlots;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(item_empty + kItemSlots);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   int *dead = const_cast<int *>(abort_flag) + 1;
   volatile int *poison = const_cast<volatile int *>(abort_flag) + 2;
@@ -220,11 +255,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = P.splits > 1 ? (int)(blockIdx.x % P.splits) : 0;
   const int n_items = P.n_tiles * P.c.heads;
-  // one item per cluster, or every gridDim.x-th
-  const int id0 = (int)blockIdx.x / P.splits, id_step = P.splits > 1 ? n_items : (int)gridDim.x;
+  // Items are dealt out in rounds over the clusters (of one CTA, where keys are not split), in alternating direction.
+  const int unit = (int)blockIdx.x / P.splits, units = (int)gridDim.x / P.splits;
+  auto id_of = [&](int r) -> int { return r * units + ((r & 1) ? units - 1 - unit : unit); };
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 2);
+    mbar_init(q_full, kQWarps);
     mbar_init(q_empty, 2);
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(&k_full[s], I8 ? 4 : 1);
@@ -235,6 +271,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     for (int s = 0; s < kScaleSlots; ++s) {
       mbar_init(&sc_full[s], 4);
       mbar_init(&sc_empty[s], 8);
+    }
+    for (int s = 0; s < kItemSlots; ++s) {
+      mbar_init(&item_full[s], 1);
+      mbar_init(&item_empty[s], kItemReaders);
     }
     for (int h = 0; h < 2; ++h) {
       mbar_init(&s_full[h], 1);
@@ -256,10 +296,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
 
   // last key that a row of the item sees
   auto last_seen = [&](const ChunkItem &it, int row) -> int {
-    return min(it.pos + (it.sub + min(row, it.rows - 1)) / P.a.group, (P.p.width << P.c.log2_page) - 1);
+    return min(it.pos + chunk_div(it.sub + min(row, it.rows - 1), P.a.group), (P.p.width << P.c.log2_page) - 1);
   };
   auto out_row = [&](const ChunkItem &it, int row) -> uint8_t * {
-    const int pr = it.sub + row, tok = pr / P.a.group;
+    const int pr = it.sub + row, tok = chunk_div(pr, P.a.group);
     return P.a.out + ((int64_t)it.token + tok) * P.a.o_row + ((int64_t)it.head * P.a.group + (pr - tok * P.a.group)) * P.a.o_head;
   };
   // Sixteen columns of a row of O from tensor memory, and, rarely, what was cleared from the values it sees given back.
@@ -298,25 +338,55 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     }
     return ok;
   };
-  if (!run) {
-  } else if (warp >= 12) {
-    if (warp > 13) {
-    // ---- Q: 64 lanes, 16-byte pieces; rows that do not exist are zeros --------------------------------------------
-    ChunkCursor cur;
-    ChunkItem it;
-    uint32_t n = 0;
-    for (int id = id0; id < n_items && !P.skip_loads && chunk_item(P, id, rank, cur, it); id += id_step) {
+  // What a role keeps from round to round: its cursors and its counts of steps, products and items.
+  ChunkCursor cur;
+  ChunkItem it, s_it;
+  uint32_t taken = 0, s_taken = 0;
+  uint32_t g = 0, n = 0, s_g = 0, s_n = 0, s_items = 0;
+  int s_j = 0;
+  bool ok = run && !(P.skip_loads && (warp == 14 || (warp >= 8 && warp < 12)));
+
+  // Alone, a CTA walks all its rounds with every role at its own pace. In a cluster the CTAs meet after each round and join.
+  for (int pass = 0;; ++pass) {
+  // The next item; false past the last. In a cluster a role does one item between two joins.
+  auto read_item = [&](uint32_t &count, ChunkItem &to, bool release) -> bool {
+    const uint32_t slot = count % kItemSlots;
+    if (!wait(&item_full[slot], (count / kItemSlots) & 1, 46)) { ok = false; return false; }
+    const int4 a = item_s[4 * slot], b = item_s[4 * slot + 1], c = item_s[4 * slot + 2];
+    if (release) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[slot]);
+    }
+    ++count;
+    to.seq = a.x; to.head = a.y; to.token = a.z; to.sub = a.w;
+    to.rows = b.x; to.pos = b.y; to.n_keys = b.z; to.first_seen = b.w;
+    to.lo = c.x; to.steps = c.y; to.n_a = c.z; to.n_b = c.w;
+    return to.seq >= 0;
+  };
+  bool first = true;
+  auto take = [&]() -> bool {
+    const bool more = ok && (P.splits == 1 || first) && read_item(taken, it, true);
+    first = false;
+    return more;
+  };
+  // ---- Q, by kQWarps warps in 16-byte pieces; rows that do not exist are zeros ----
+  auto load_q = [&](int w) {
+    constexpr int kUnits = D / 8, kRows = kQWarps * 32 / kUnits;  // pieces of a row; rows at once
+    const int u = (w * 32 + lane) % kUnits, step_tok = chunk_div(kRows, P.a.group), step_head = kRows - step_tok * P.a.group;
+    while (take()) {
       if (it.steps == 0) continue;
-      if (!wait(q_empty, (n & 1) ^ 1, 32)) break;
+      if (!(ok = wait(q_empty, (n & 1) ^ 1, 32))) break;
       ++n;
-      constexpr int kUnits = D / 8;
-      for (int i = (warp - 14) * 32 + lane; i < kChunkRows * kUnits; i += 64) {
-        const int r = i / kUnits, u = i % kUnits;
-        const bool in = r < it.rows;
-        const int pr = it.sub + (in ? r : 0), tok = pr / P.a.group, g = pr - tok * P.a.group;
-        const uint8_t *src = P.a.q + ((int64_t)it.token + tok) * P.a.q_row + ((int64_t)it.head * P.a.group + g) * P.a.q_head + u * 16;
-        const uint32_t dst = smem_u32(q_s) + (r >> 7) * (S::kQ / 2) + (u >> 3) * 16384 + (r & 127) * 128 + (((u & 7) ^ (r & 7)) << 4);
+      int row = (w * 32 + lane) / kUnits;
+      int tok = chunk_div(it.sub + row, P.a.group), head = it.sub + row - tok * P.a.group;
+      for (; row < kChunkRows; row += kRows) {
+        const bool in = row < it.rows;
+        const uint8_t *src = P.a.q + ((int64_t)it.token + (in ? tok : 0)) * P.a.q_row + ((int64_t)it.head * P.a.group + (in ? head : 0)) * P.a.q_head + u * 16;
+        const uint32_t dst = smem_u32(q_s) + (row >> 7) * (S::kQ / 2) + (u >> 3) * 16384 + (row & 127) * 128 + (((u & 7) ^ (row & 7)) << 4);
         chunk_copy16(dst, src, in);
+        tok += step_tok;
+        head += step_head;
+        if (head >= P.a.group) { head -= P.a.group; ++tok; }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
       asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -324,6 +394,29 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
+  };
+  if (!run) {
+  } else if (warp >= 12) {
+    if (warp == 15) {
+      for (bool more = true; more && ok; ++taken) {
+        const int id = id_of((int)taken);
+        more = id < n_items && chunk_item(P, id, rank, cur, it);
+        const uint32_t slot = taken % kItemSlots;
+        if (!(ok = wait(&item_empty[slot], ((taken / kItemSlots) & 1) ^ 1, 47))) break;
+        if (lane == 0) {
+          item_s[4 * slot] = make_int4(more ? it.seq : -1, it.head, it.token, it.sub);
+          item_s[4 * slot + 1] = make_int4(it.rows, it.pos, it.n_keys, it.first_seen);
+          item_s[4 * slot + 2] = make_int4(it.lo, it.steps, it.n_a, it.n_b);
+          mbar_arrive(&item_full[slot]);
+        }
+        __syncwarp();
+        if (P.splits > 1) {  // one between two joins
+          ++taken;
+          break;
+        }
+      }
+    } else if (warp == 14) {
+      load_q(0);
     } else {
     // ---- MMA of one half ----------------------------------------------------------------------------------------------
     // A half that has nothing in a step still waits for the step's operands before it gives them up: its arrivals must not
@@ -332,19 +425,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     const uint32_t idesc_s = attn_idesc(HALF, false, 128), idesc_pv = attn_idesc(HALF, true, D);
     const uint32_t t_s = tmem + h * 128, t_p = S::kAhead ? tmem + 384 + h * 64 : t_s, t_o = tmem + 256 + h * D;
     const uint32_t q_at = smem_u32(q_s) + h * (S::kQ / 2);
-    ChunkCursor s_cur, cur;
-    ChunkItem s_it, it;
-    int s_id = id0, s_j = 0;
-    bool s_more = false;
+    bool s_more = false, s_first = true;
     auto s_seek = [&]() {  // the next item with blocks for this CTA
-      s_more = false;
-      for (; s_id < n_items; s_id += id_step) {
-        if (!chunk_item(P, s_id, rank, s_cur, s_it)) return;
-        if (s_it.steps > 0) { s_more = true; return; }
-      }
+      do {
+        s_more = ok && (P.splits == 1 || s_first) && read_item(s_taken, s_it, false);
+        s_first = false;
+      } while (s_more && s_it.steps == 0);
     };
     s_seek();
-    uint32_t s_g = 0, s_items = 0, s_n = 0, g = 0, n = 0;
     // scores of the step at the S cursor, one step ahead of the products
     auto issue_s = [&]() -> bool {
       if (s_j == 0 && !wait(q_full, s_items & 1, 34)) return false;
@@ -380,13 +468,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       if (++s_j == s_it.steps) {
         ++s_items;
         s_j = 0;
-        s_id += id_step;
         s_seek();
       }
       return true;
     };
-    bool ok = !s_more || issue_s();
-    for (int id = id0; id < n_items && ok && chunk_item(P, id, rank, cur, it); id += id_step) {
+    ok = ok && (!s_more || issue_s());
+    while (take()) {
       for (int j = 0; j < it.steps && ok; ++j, ++g) {
         if (S::kAhead && s_more && !(ok = issue_s())) break;
         const uint32_t vs = g % S::kStages, ph = (g / S::kStages) & 1;
@@ -413,14 +500,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     }
   } else if (warp >= 8) {
     // ---- keys and values --------------------------------------------------------------------------------------------
-    ChunkCursor cur;
-    ChunkItem it;
-    uint32_t g = 0;
-    bool ok = !P.skip_loads;
     if constexpr (!I8) {
       if (warp == 8) {
         const int per = 128 >> P.c.log2_page;  // pages of a block, a lane each
-        for (int id = id0; id < n_items && ok && chunk_item(P, id, rank, cur, it); id += id_step) {
+        while (take()) {
           auto page_of = [&](int j) -> int {
             const int pos = ((it.lo + j) << 7) + (lane << P.c.log2_page);
             const int page = lane < per && pos < it.n_keys ? kv_page(P.p, P.c, it.seq, pos) : -1;
@@ -447,13 +530,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
             page = next;
           }
         }
+      } else {
+        load_q(warp - 8);  // 1 to 3: an int8 cache needs these warps for its keys
       }
     } else {
       constexpr int kChunks = D / 16;         // 16-byte pieces of a key
       constexpr int kKeys = 32 / kChunks;     // keys that the warp's lanes reach at once
       const int w = warp - 8, key = w * 32 + lane;
       const uint32_t raw = smem_u32(raw_s) + w * 32 * D;
-      for (int id = id0; id < n_items && ok && chunk_item(P, id, rank, cur, it); id += id_step) {
+      while (take()) {
         // this lane's key of step j: its page, or -1
         auto page_of = [&](int j) -> int {
           const int pos = ((it.lo + j) << 7) + key;
@@ -544,11 +629,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     const uint32_t p_addr = tmem + lanes + (S::kAhead ? 384 + h * 64 : h * 128);
     const float c = P.a.c;
     const float2 c2 = make_float2(c, c);
-    uint32_t g = 0, n = 0;
-    bool ok = true;
-    ChunkCursor cur;
-    ChunkItem it;
-    for (int id = id0; id < n_items && chunk_item(P, id, rank, cur, it); id += id_step) {
+    while (take()) {
       // last key that this row sees, and the warp's first row; rows that do not exist see what the last one does
       const int lim = last_seen(it, row);
       const int warp_lim = __shfl_sync(0xffffffffu, lim, 0);
@@ -791,27 +872,32 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
 
   tc_fence_before();
   __syncthreads();
-  if (P.splits == 1) {
-    if (warp == 12) tmem_dealloc(tmem, 512);
-    return;
+  if (P.splits == 1) break;
+  // The round's item once more, for the warps whose role did not read it. A CTA whose wait ran out writes nothing, but stays
+  // for every barrier of its cluster, since the others read its shared memory.
+  const bool good = run && *abort_flag == 0;
+  {
+    const int4 a = item_s[4 * (pass % kItemSlots)], b = item_s[4 * (pass % kItemSlots) + 1], c = item_s[4 * (pass % kItemSlots) + 2];
+    it.seq = a.x; it.head = a.y; it.token = a.z; it.sub = a.w;
+    it.rows = b.x; it.pos = b.y; it.n_keys = b.z; it.first_seen = b.w;
+    it.lo = c.x; it.steps = c.y; it.n_a = c.z; it.n_b = c.w;
   }
+  if (good ? it.seq < 0 : id_of(pass) >= n_items) break;
 
   // ---- join the CTAs of the cluster ---------------------------------------------------------------------------------------
-  // Every role is done, so the rings are free: they take the partial rows, by columns of four, so that neighbouring rows fall
-  // into neighbouring banks.
+  // Every role is done with the item, so the rings are free: they take the partial rows, by columns of four, so that
+  // neighbouring rows fall into neighbouring banks.
   tc_fence_after();
-  ChunkCursor cur;
-  ChunkItem it;
-  const bool good = run && *abort_flag == 0 && id0 < n_items && chunk_item(P, id0, rank, cur, it);
   if (good && warp < 8) {
     const int row = threadIdx.x, h = warp >> 2;
     const bool any = it.blocks(h) > 0, seen = any && ml_s[row] != -INFINITY;
     const uint32_t o_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 256 + h * D;
     const int lim = last_seen(it, row);
-#pragma unroll 1
+    const bool slow = !I8 && any && *poison != 0;
+#pragma unroll 2
     for (int q4 = 0; q4 < D / 16; ++q4) {
       float o[16];
-      load_o(it, o_addr, q4, any, seen, !I8 && any && *poison != 0, lim, o);
+      load_o(it, o_addr, q4, any, seen, slow, lim, o);
       float4 *st = reinterpret_cast<float4 *>(k_s) + q4 * 4 * kChunkRows + row;
 #pragma unroll
       for (int i = 0; i < 4; ++i) st[i * kChunkRows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
@@ -819,59 +905,123 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
   }
   tc_fence_before();
   chunk_cluster_sync();
-  if (warp == 12) tmem_dealloc(tmem, 512);
-  if (good) {  // each CTA writes its share of the rows
-    constexpr int kParts = D / 8;  // eight values of a row per thread
-    const int r0 = kChunkRows * rank / P.splits, r1 = min(kChunkRows * (rank + 1) / P.splits, it.rows);
-    for (int i = (int)threadIdx.x + r0 * kParts; i < r1 * kParts; i += kChunkThreads) {
-      const int row = i / kParts, part = i % kParts;
-      float mm = -INFINITY;
-      for (int s = 0; s < P.splits; ++s) mm = fmaxf(mm, chunk_peer(smem_u32(ml_s + row), s));
-      float o[8] = {}, sum = 0.f;
-      if (mm != -INFINITY) {
-        for (int s = 0; s < P.splits; ++s) {
-          const float e = ex2f(chunk_peer(smem_u32(ml_s + row), s) - mm);
-          sum += chunk_peer(smem_u32(ml_s + kChunkRows + row), s) * e;
-          const uint32_t at = smem_u32(k_s) + ((part * 2) * kChunkRows + row) * 16;
-          const float4 x = chunk_peer4(at, s), y = chunk_peer4(at + kChunkRows * 16, s);
-          o[0] += x.x * e; o[1] += x.y * e; o[2] += x.z * e; o[3] += x.w * e;
-          o[4] += y.x * e; o[5] += y.y * e; o[6] += y.z * e; o[7] += y.w * e;
-        }
+  // each CTA writes its share of the rows: first how much each part counts, then the weighted sums, eight values a thread
+  auto join = [&](auto parts) {
+    constexpr int N = decltype(parts)::value, kShare = kChunkRows / N, kParts = D / 8;
+    float *weight = ml_s + 2 * kChunkRows;
+    const int r0 = rank * kShare, n_rows = min(kShare, it.rows - r0);
+    if (threadIdx.x < kChunkRows) {
+      const int row = threadIdx.x % kShare, part = threadIdx.x / kShare;
+      float pm[N], pl[N], mm = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int s = 0; s < N; ++s) {
+        pm[s] = chunk_peer(smem_u32(ml_s + r0 + row), s);
+        pl[s] = chunk_peer(smem_u32(ml_s + kChunkRows + r0 + row), s);
       }
-      const float inv = mm != -INFINITY ? 1.0f / sum : 0.f;
-      *reinterpret_cast<uint4 *>(out_row(it, row) + part * 16) = make_uint4(out_pair<HALF>(o[0] * inv, o[1] * inv), out_pair<HALF>(o[2] * inv, o[3] * inv),
-                                                               out_pair<HALF>(o[4] * inv, o[5] * inv), out_pair<HALF>(o[6] * inv, o[7] * inv));
+#pragma unroll
+      for (int s = 0; s < N; ++s) mm = fmaxf(mm, pm[s]);
+      float mine = 0.f;
+#pragma unroll
+      for (int s = 0; s < N; ++s) {
+        const float e = pm[s] == -INFINITY ? 0.f : ex2f(pm[s] - mm);
+        sum += pl[s] * e;
+        if (s == part) mine = e;
+      }
+      weight[part * kShare + row] = mm == -INFINITY ? 0.f : mine / sum;
     }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_rows * kParts; i += kChunkThreads) {
+      const int row = i / kParts, part = i % kParts;
+      const uint32_t at = smem_u32(k_s) + ((part * 2) * kChunkRows + r0 + row) * 16;
+      float4 x[N], y[N];
+#pragma unroll
+      for (int s = 0; s < N; ++s) {
+        x[s] = chunk_peer4(at, s);
+        y[s] = chunk_peer4(at + kChunkRows * 16, s);
+      }
+      float o[8] = {};
+#pragma unroll
+      for (int s = 0; s < N; ++s) {
+        const float e = weight[s * kShare + row];
+        o[0] += x[s].x * e; o[1] += x[s].y * e; o[2] += x[s].z * e; o[3] += x[s].w * e;
+        o[4] += y[s].x * e; o[5] += y[s].y * e; o[6] += y[s].z * e; o[7] += y[s].w * e;
+      }
+      *reinterpret_cast<uint4 *>(out_row(it, r0 + row) + part * 16) =
+          make_uint4(out_pair<HALF>(o[0], o[1]), out_pair<HALF>(o[2], o[3]), out_pair<HALF>(o[4], o[5]), out_pair<HALF>(o[6], o[7]));
+    }
+  };
+  if (good) {
+    if (P.splits == 2) join(std::integral_constant<int, 2>{});
+    else if (P.splits == 4) join(std::integral_constant<int, 4>{});
+    else join(std::integral_constant<int, 8>{});
   }
-  chunk_cluster_sync();  // nobody's shared memory goes away while it is read
+  fence_proxy_async();   // TMA may write next where the partial rows lay
+  chunk_cluster_sync();  // nobody's shared memory changes or goes away while it is read
+  }
+  if (warp == 12) tmem_dealloc(tmem, 512);
 }
 
 template <bool HALF, int D, bool I8>
-static int launch(const ChunkParams &P, const CUtensorMap &mk, const CUtensorMap &mv, unsigned grid, cudaStream_t stream) {
+static int launch(ChunkParams &P, const CUtensorMap &mk, const CUtensorMap &mv, int64_t items, int64_t blocks, cudaStream_t stream) {
   using S = ChunkTile<D, I8>;
   const auto kernel = paged_chunk_kernel<HALF, D, I8>;
-  // the attribute belongs to the device: set once on each, again where two threads meet
-  static std::atomic<bool> ready[64];
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-    if (e != cudaSuccess) {
-      set_error(std::string("paged_attention: cannot raise the shared-memory limit: ") + cudaGetErrorString(e));
-      return PGB_ERR_CUDA;
-    }
-    if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_relaxed);
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    set_error("paged_attention: cannot tell the current device");
+    return PGB_ERR_CUDA;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kChunkThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = P.splits;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  // Per device: the shared-memory limit is raised, and how many clusters of 2, 4 and 8 run at a time is asked for, once; again
+  // where two threads meet. The processor clusters' SMs do not divide evenly: 148 SMs hold fewer than 148 / 4 clusters of
+  // four, and one cluster too many would wait for a whole round of the others.
+  static std::atomic<uint32_t> capacity[64];
+  uint32_t cap = capacity[dev].load(std::memory_order_relaxed);
+  if (cap == 0) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    for (int k = 3; k >= 1 && e == cudaSuccess; --k) {
+      int n = 0;
+      attr[0].val.clusterDim.x = 1u << k;
+      cfg.gridDim = dim3(1u << k);
+      e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+      cap = cap << 8 | (uint32_t)std::min(n, 255);
+    }
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      set_error(std::string("paged_attention: cannot set up the kernel: ") + cudaGetErrorString(e));
+      return PGB_ERR_CUDA;
+    }
+    cap |= 1u << 31;
+    capacity[dev].store(cap, std::memory_order_relaxed);
+  }
+  // CTAs per item: what makes the launch shortest, in steps of a block of keys. Of s CTAs' share of the longest item and of
+  // all items (which have, by and large, 0.6 of the longest's keys) over the clusters that run at once, the longer counts;
+  // each round costs one and a half steps to fill and drain, and four where CTAs join (12 heads of 64, contexts of 5003 and
+  // 3000 int8 tokens, 36 items: 74, 49 and 53 us with 2, 4 and 8 CTAs).
+  P.splits = 1;
+  int64_t units = sm_count();
+  double best = 0;
+  for (int k = 0; k <= 3; ++k) {
+    const int64_t s = 1 << k, n = k == 0 ? sm_count() : (cap >> (8 * (k - 1))) & (k == 3 ? 127 : 255);
+    if (n == 0 || (k > 0 && blocks < 2 * s)) continue;
+    const double part = (double)blocks / s, rounds = std::max(1.0, (double)items / n);
+    const double t = std::max(part, 0.6 * part * items / n) + rounds * (k ? 4.0 : 1.5);
+    if (k == 0 || t < best) {
+      best = t;
+      P.splits = (int)s;
+      units = n;
+    }
+  }
+  cfg.gridDim = dim3((unsigned)(std::min(items, units) * P.splits));
+  attr[0].val.clusterDim.x = P.splits;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mk, mv, P);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -909,8 +1059,6 @@ bool run_paged_chunk(const PagedParams &a, const KvCache &c, const KvPlan &p, bo
   if (c.dtype != PGB_I8 && (!page_map(&mk, c, c.k) || !page_map(&mv, c, c.v))) return false;
   P.n_tiles = (int)tiles;
   const int64_t items = tiles * c.heads, blocks = ((int64_t)p.width << c.log2_page) / 128;
-  P.splits = 1;
-  while (P.splits < 8 && items * P.splits * 2 <= sm_count() && blocks >= 4LL * P.splits) P.splits *= 2;
   P.err = gemm_error_word();
   if (!P.err) {
     set_error("paged_attention: cannot resolve the device error word");
@@ -920,9 +1068,8 @@ bool run_paged_chunk(const PagedParams &a, const KvCache &c, const KvPlan &p, bo
   uint32_t drill_polls = 0;
   take_next_wait_test(&drill_polls, &P.skip_loads);
   P.polls = drill_polls ? drill_polls : kChunkPolls;
-  const unsigned grid = P.splits > 1 ? (unsigned)(items * P.splits) : (unsigned)std::min<int64_t>(items, sm_count());
   const bool i8 = c.dtype == PGB_I8;
-#define PGB_CHUNK(H, D, Q) launch<H, D, Q>(P, mk, mv, grid, stream)
+#define PGB_CHUNK(H, D, Q) launch<H, D, Q>(P, mk, mv, items, blocks, stream)
   if (half) {
     if (c.head_dim == 64) *status = i8 ? PGB_CHUNK(true, 64, true) : PGB_CHUNK(true, 64, false);
     else *status = i8 ? PGB_CHUNK(true, 128, true) : PGB_CHUNK(true, 128, false);
