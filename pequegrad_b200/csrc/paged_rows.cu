@@ -11,10 +11,10 @@
 //            columns of the output likewise, so both products take their operands as they lie in memory.
 //   softmax  running maximum and sum per row in fp32; the warps' and then the CTAs' partial results are joined in shared and
 //            distributed shared memory, in a fixed order. No scratch in global memory, nothing shared between launches.
-//   int8     widened exactly to 16 bits; the key's scale multiplies its scores, the value's scale its probabilities, in fp32.
-//            For fp16 queries the scaled probabilities, whose range fp16 does not have, go in as two bf16 terms.
+//   int8     widened exactly to fp16; the key's scale multiplies its scores, the value's scale its probabilities, in fp32.
 #include <atomic>
 #include <string>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -57,6 +57,11 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool HALF>
+__device__ __forceinline__ bool not_finite(uint32_t bits) {  // of one 16-bit float
+  constexpr uint32_t e = HALF ? 0x7c00u : 0x7f80u;
+  return (bits & e) == e;
 }
 __device__ __forceinline__ uint4 ld_shared16(uint32_t a) {
   uint4 r;
@@ -101,22 +106,26 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) paged_rows_kernel(const __g
   const int heads_here = min(a.group - sub * 16, 16);
   const int n_tok = (int)min((int64_t)tokens, end - row0);
   const int n_rows = n_tok * heads_here;
-  const int64_t held = (int64_t)p.width << c.log2_page;
-  const int64_t pos0 = kv_position(p, seq, row0);
-  const int64_t n_keys = max((int64_t)0, min(pos0 + n_tok, held));  // what the tile's last token sees
-  const int64_t n_blocks = (n_keys + 15) >> 4;
+  const int held = p.width << c.log2_page;  // at most 2^30
+  const int pos0 = (int)max(kv_position(p, seq, row0), -((int64_t)1 << 31));
+  const int n_keys = max(0, min(held, pos0 + n_tok));  // what the tile's last token sees
+  const int n_blocks = (n_keys + 15) >> 4;
 
   // Q in the order in which the chunks of K arrive: value i of this lane's D / 4 is d = 16/es * (t + 4 (i es / 16)) + ...
+  // Beside an int8 cache the products run in fp16: there a key widens in fewer steps than in bf16. A bf16 row of Q is brought
+  // into fp16's range by a power of two, exactly but for values 2^-29 of the row's largest; its scores are scaled back.
+  constexpr bool kHalfMma = HALF || I8;
   constexpr int kPer = 16 / S::kEs;  // values in a 16-byte chunk of K
   uint32_t q[D / 16][4];
-  int64_t lim[2];  // last key that the lane's two rows see
+  int lim[2];      // last key that the lane's two rows see
+  float scale[2];  // of their scores
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int i = quad + 8 * h;
     const int tok = i / heads_here, head = i - tok * heads_here;
-    lim[h] = min(pos0 + tok, held - 1);
     const bool in = i < n_rows;
-    if (!in) lim[h] = -1;
+    lim[h] = in ? min(pos0 + tok, held - 1) : -1;
+    scale[h] = a.c;
     const uint8_t *src = a.q + (row0 + (in ? tok : 0)) * a.q_row + ((int64_t)kvh * a.group + sub * 16 + (in ? head : 0)) * a.q_head;
 #pragma unroll
     for (int j = 0; j < S::kKChunks; ++j) {
@@ -129,44 +138,70 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) paged_rows_kernel(const __g
         q[s + 1][h] = r.z; q[s + 1][2 + h] = r.w;
       }
     }
+    if constexpr (I8 && !HALF) {
+      uint32_t top = 0;  // largest |q| as bf16 bits
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) top = max(top, max(q[s][2 * e + h] & 0x7fffu, (q[s][2 * e + h] >> 16) & 0x7fffu));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int up = min(14 + 127 - (int)(top >> 7), 100);  // the largest value lands in [2^14, 2^15)
+      const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+      scale[h] *= __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t &w = q[s][2 * e + h];
+          w = paged_pack<true>(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xffff0000u) * f);
+        }
+    }
   }
-  const int64_t lim_min = pos0;  // the tile's first token: keys up to here are seen by all its rows
+  const int lim_min = pos0;  // the tile's first token: keys up to here are seen by all its rows
 
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem) + warp * S::kWarp;
-  const int64_t step = (int64_t)splits * kRowWarps;
-  const int64_t block0 = (int64_t)rank * kRowWarps + warp;
-  auto page_of = [&](int64_t kb) -> int { return kb < n_blocks ? kv_page(p, c, seq, kb << 4) : -1; };
+  const int step = (int)splits * kRowWarps, block0 = rank * kRowWarps + warp, page_mask = (1 << c.log2_page) - 1;
+  const int *table = p.table + (int64_t)seq * p.pitch;
+  const uint8_t *k_head = c.k.base + kvh * c.k.head + quad * c.k.slot + t * 16, *v_head = c.v.base + kvh * c.v.head + 2 * t * c.v.slot + quad * S::kVPiece;
+  // the table's entry for block kb; looked up long before it is judged
+  auto entry_of = [&](int kb) -> int { return kb < n_blocks ? __ldg(table + (kb >> (c.log2_page - 4))) : -1; };
   // Starts the copies of block kb (of the page given) into a stage. What the lane copies is what it reads.
-  auto fetch = [&](int64_t kb, int page, int stage) {
+  auto fetch = [&](int kb, int page, int stage) {
     if (kb < n_blocks) {
       const uint32_t dst = base + stage * S::kStage;
-      const int slot0 = (int)((kb << 4) & ((1 << c.log2_page) - 1));
-      const int there = page < 0 ? 0 : (int)min((int64_t)16, n_keys - (kb << 4));  // keys of the block that exist
-      const int64_t pg = page < 0 ? 0 : page;
-      const uint8_t *k = c.k.base + pg * c.k.page + kvh * c.k.head + slot0 * c.k.slot;
-      const uint8_t *v = c.v.base + pg * c.v.page + kvh * c.v.head + slot0 * c.v.slot;
+      const int slot0 = (kb << 4) & page_mask;
+      const bool ok = (unsigned)page < (unsigned)c.n_pages;
+      const int64_t pg = ok ? page : 0;
+      const int there = ok ? n_keys - (kb << 4) : 0;  // keys of the block that exist, if fewer than 16
+      const uint8_t *k = k_head + pg * c.k.page + slot0 * c.k.slot, *v = v_head + pg * c.v.page + slot0 * c.v.slot;
+      auto pieces = [&](auto whole) {
+        constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int key = quad + 8 * h;
+        for (int h = 0; h < 2; ++h) {
+          const bool in = kWhole || quad + 8 * h < there;
 #pragma unroll
-        for (int j = 0; j < S::kKChunks; ++j)
-          copy16(dst + ((h * S::kKChunks + j) * 32 + lane) * 16, key < there ? k + key * c.k.slot + (t + 4 * j) * 16 : c.k.base, key < there);
-      }
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int key = 2 * t + (g & 1) + 8 * (g >> 1);
-#pragma unroll
-        for (int j = 0; j < S::kVPieces; ++j) {
-          const uint32_t to = dst + S::kK + ((g * S::kVPieces + j) * 32 + lane) * S::kVPiece;
-          const uint8_t *from = key < there ? v + key * c.v.slot + (quad + 8 * j) * S::kVPiece : c.v.base;
-          if (S::kVPiece == 16) copy16(to, from, key < there);
-          else copy8(to, from, key < there);
+          for (int j = 0; j < S::kKChunks; ++j)
+            copy16(dst + ((h * S::kKChunks + j) * 32 + lane) * 16, in ? k + h * 8 * c.k.slot + j * 64 : c.k.base, in);
         }
-      }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const bool in = kWhole || 2 * t + (g & 1) + 8 * (g >> 1) < there;
+#pragma unroll
+          for (int j = 0; j < S::kVPieces; ++j) {
+            const uint32_t to = dst + S::kK + ((g * S::kVPieces + j) * 32 + lane) * S::kVPiece;
+            const uint8_t *from = in ? v + ((g & 1) + 8 * (g >> 1)) * c.v.slot + j * 8 * S::kVPiece : c.v.base;
+            if (S::kVPiece == 16) copy16(to, from, in);
+            else copy8(to, from, in);
+          }
+        }
+      };
+      if (there >= 16) pieces(std::true_type{});
+      else pieces(std::false_type{});
       if (I8 && lane < 8) {  // scales of the block: slots are contiguous, 16 of them 16-byte aligned
         const KvPages &w = lane < 4 ? c.k : c.v;
         const float *s = w.scale + pg * w.scale_page + kvh * w.scale_head + slot0 + (lane & 3) * 4;
-        copy16(dst + S::kK + S::kV + lane * 16, page < 0 ? w.scale : s, page >= 0);
+        copy16(dst + S::kK + S::kV + lane * 16, s, ok);
       }
     }
     copy_commit();  // empty groups keep the count
@@ -175,20 +210,22 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) paged_rows_kernel(const __g
   float o[D / 8][4];
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  // Reference of the exponents: m + lv. lv is the power of two of the value scales met so far: the scaled probabilities then
+  // stay within fp16, and since it is the same for all rows and in the sums too, O / l is what it was.
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, lv = I8 ? -100.f : 0.f;
 
-  int pages[S::kStages];  // of the blocks under way
+  int pages[S::kStages];  // table entries of the blocks under way
 #pragma unroll
-  for (int i = 0; i < S::kStages; ++i) pages[i] = page_of(block0 + i * step);
+  for (int i = 0; i < S::kStages; ++i) pages[i] = entry_of(block0 + i * step);
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) fetch(block0 + i * step, pages[i], i);
   int stage = 0;
-  for (int64_t kb = block0; kb < n_blocks; kb += step) {
-    const int page = pages[0];
+  for (int kb = block0; kb < n_blocks; kb += step) {
+    const bool absent = (unsigned)pages[0] >= (unsigned)c.n_pages;
     fetch(kb + (S::kStages - 1) * step, pages[S::kStages - 1], stage == 0 ? S::kStages - 1 : stage - 1);
 #pragma unroll
     for (int i = 0; i + 1 < S::kStages; ++i) pages[i] = pages[i + 1];
-    pages[S::kStages - 1] = page_of(kb + S::kStages * step);
+    pages[S::kStages - 1] = entry_of(kb + S::kStages * step);
     copy_wait<S::kStages - 1>();
     if (I8) __syncwarp();  // the scales were copied by other lanes
     const uint32_t src = base + stage * S::kStage;
@@ -203,37 +240,39 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) paged_rows_kernel(const __g
         if constexpr (I8) {
           const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mma16816<HALF>(s[h], q[4 * j + e], paged_widen2<HALF>(w[e], 0), paged_widen2<HALF>(w[e], 1));
+          for (int e = 0; e < 4; ++e) mma16816<true>(s[h], q[4 * j + e], paged_widen2<true>(w[e], 0), paged_widen2<true>(w[e], 1));
         } else {
           mma16816<HALF>(s[h], q[2 * j], r.x, r.y);
           mma16816<HALF>(s[h], q[2 * j + 1], r.z, r.w);
         }
       }
     }
+    const int key0 = kb << 4;
+    const bool masked = key0 + 15 > lim_min || absent;  // warp-uniform
     float vs[4];
-    {
-      float ks[4] = {a.c, a.c, a.c, a.c};
-      if constexpr (I8) {
-        const uint32_t at = src + S::kK + S::kV + 8 * t;
-        const uint2 k0 = ld_shared8(at), k1 = ld_shared8(at + 32), v0 = ld_shared8(at + 64), v1 = ld_shared8(at + 96);
-        ks[0] *= __uint_as_float(k0.x); ks[1] *= __uint_as_float(k0.y); ks[2] *= __uint_as_float(k1.x); ks[3] *= __uint_as_float(k1.y);
-        vs[0] = __uint_as_float(v0.x); vs[1] = __uint_as_float(v0.y); vs[2] = __uint_as_float(v1.x); vs[3] = __uint_as_float(v1.y);
-      }
+    if constexpr (I8) {
+      const uint32_t at = src + S::kK + S::kV + 8 * t;
+      const uint2 k0 = ld_shared8(at), k1 = ld_shared8(at + 32), v0 = ld_shared8(at + 64), v1 = ld_shared8(at + 96);
+      const float ks[4] = {__uint_as_float(k0.x), __uint_as_float(k0.y), __uint_as_float(k1.x), __uint_as_float(k1.y)};
+      vs[0] = __uint_as_float(v0.x); vs[1] = __uint_as_float(v0.y); vs[2] = __uint_as_float(v1.x); vs[3] = __uint_as_float(v1.y);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[h][e] *= ks[2 * h + (e & 1)];
     }
-    const int64_t key0 = kb << 4;
-    if (key0 + 15 > lim_min || page < 0) {  // warp-uniform
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[h][e] *= scale[e >> 1];
+    if (masked) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int64_t key = key0 + 8 * h + 2 * t + (e & 1);
-          if (key > lim[e >> 1] || page < 0) s[h][e] = -INFINITY;
+          const int key = key0 + 8 * h + 2 * t + (e & 1);
+          if (key > lim[e >> 1] || absent) s[h][e] = -INFINITY;
           // a slot behind the context has a stale scale: its probability of zero must meet a number
-          if (I8 && e < 2 && (key >= n_keys || page < 0)) vs[2 * h + e] = 0.f;
+          if (I8 && e < 2 && (key >= n_keys || absent)) vs[2 * h + e] = 0.f;
         }
     }
     float mx[2];
@@ -243,50 +282,67 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) paged_rows_kernel(const __g
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
     }
-    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {  // rare once the largest scores have been met
+    float lv_new = lv;
+    if constexpr (I8) {
+      float top = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t e = __float_as_uint(top) >> 23;
+      if (e < 255) lv_new = fmaxf(lv, (float)(int)e - 127.f);
+    }
+    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1] || lv_new != lv)) {  // rare once the largest scores have been met
       float alpha[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const float mn = fmaxf(m[r], mx[r]);
-        alpha[r] = mn == -INFINITY ? 1.f : paged_ex2(m[r] - mn);
+        alpha[r] = mn == -INFINITY ? 1.f : paged_ex2(m[r] - mn + (lv - lv_new));
         m[r] = mn;
         l[r] *= alpha[r];
       }
+      lv = lv_new;
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) {
         o[i][0] *= alpha[0]; o[i][1] *= alpha[0];
         o[i][2] *= alpha[1]; o[i][3] *= alpha[1];
       }
     }
-    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[h][e] = paged_ex2(s[h][e] - ref[e >> 1]);
-        l[e >> 1] += s[h][e];
-      }
+    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0] + lv, m[1] == -INFINITY ? 0.f : m[1] + lv};
     // The probabilities as the A operand of the second product: the accumulator's layout is the operand's.
-    constexpr bool kTwoTerms = I8 && HALF;
-    constexpr bool kPHalf = HALF && !I8;
-    uint32_t pa[4], pb[4];
+    uint32_t pa[4];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float x = s[h][2 * r], y = s[h][2 * r + 1];
-        if (I8) { x *= vs[2 * h]; y *= vs[2 * h + 1]; }
-        pa[2 * h + r] = paged_pack<kPHalf>(x, y);
-        if (kTwoTerms) {
-          const float xr = x - __uint_as_float(pa[2 * h + r] << 16), yr = y - __uint_as_float(pa[2 * h + r] & 0xffff0000u);
-          pb[2 * h + r] = paged_pack<false>(xr, yr);
+        float x = paged_ex2(s[h][2 * r] - ref[r]), y = paged_ex2(s[h][2 * r + 1] - ref[r]);
+        l[r] += x + y;
+        if (I8) {  // a token that a row does not see may have a scale that is no number
+          x = x == 0.f ? 0.f : x * vs[2 * h];
+          y = y == 0.f ? 0.f : y * vs[2 * h + 1];
         }
+        pa[2 * h + r] = paged_pack<kHalfMma>(x, y);
       }
     const uint32_t vsrc = src + S::kK + lane * S::kVPiece;
+    bool cleared = false;
     auto value_words = [&](int g, int j) -> uint4 {
       const uint32_t at = vsrc + (g * S::kVPieces + j) * 32 * S::kVPiece;
-      if constexpr (S::kVPiece == 16) return ld_shared16(at);
-      else { const uint2 r = ld_shared8(at); return make_uint4(r.x, r.y, 0, 0); }
+      if constexpr (S::kVPiece == 16) {
+        uint4 r = ld_shared16(at);
+        // A new token that some rows must not see: NaN and infinities would reach them through a probability of zero.
+        if (!I8 && masked && key0 + 2 * t + (g & 1) + 8 * (g >> 1) > lim_min) {
+          uint32_t *w = reinterpret_cast<uint32_t *>(&r);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool lo = not_finite<HALF>(w[e] & 0xffffu), hi = not_finite<HALF>(w[e] >> 16);
+            if (lo) w[e] &= 0xffff0000u;
+            if (hi) w[e] &= 0xffffu;
+            cleared |= lo || hi;
+          }
+        }
+        return r;
+      } else {
+        const uint2 r = ld_shared8(at);
+        return make_uint4(r.x, r.y, 0, 0);
+      }
     };
 #pragma unroll
     for (int j = 0; j < S::kVPieces; ++j) {
@@ -300,16 +356,33 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) paged_rows_kernel(const __g
           const uint32_t lo01 = __byte_perm(w0[e], w1[e], 0x5140), hi01 = __byte_perm(w0[e], w1[e], 0x7362);
           const uint32_t lo23 = __byte_perm(w2[e], w3[e], 0x5140), hi23 = __byte_perm(w2[e], w3[e], 0x7362);
 #pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            const uint32_t b0 = paged_widen2<kPHalf>(d < 2 ? lo01 : hi01, d & 1), b1 = paged_widen2<kPHalf>(d < 2 ? lo23 : hi23, d & 1);
-            float(&acc)[4] = o[j * kWords * 4 + 4 * e + d];
-            mma16816<kPHalf>(acc, pa, b0, b1);
-            if (kTwoTerms) mma16816<kPHalf>(acc, pb, b0, b1);
-          }
+          for (int d = 0; d < 4; ++d)
+            mma16816<true>(o[j * kWords * 4 + 4 * e + d], pa, paged_widen2<true>(d < 2 ? lo01 : hi01, d & 1), paged_widen2<true>(d < 2 ? lo23 : hi23, d & 1));
         } else {
           mma16816<HALF>(o[j * 8 + 2 * e], pa, __byte_perm(w0[e], w1[e], 0x5410), __byte_perm(w2[e], w3[e], 0x5410));
           mma16816<HALF>(o[j * 8 + 2 * e + 1], pa, __byte_perm(w0[e], w1[e], 0x7632), __byte_perm(w2[e], w3[e], 0x7632));
         }
+      }
+    }
+    if constexpr (!I8) {
+      if (masked && __any_sync(0xffffffffu, cleared)) {  // rare: give back what was cleared, to the rows that see it
+        __syncwarp();                                    // the values lie in other lanes' slots
+        for (int key = max(0, lim_min + 1 - key0); key < min(16, n_keys - key0); ++key) {
+          const int g = (key & 1) + 2 * (key >> 3), owner = (key & 7) >> 1;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t at = src + S::kK + ((g * S::kVPieces + i / 8) * 32 + (2 * t + e) * 4 + owner) * 16 + 2 * (i % 8);
+              unsigned short bits;
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(at) : "memory");
+              if (!not_finite<HALF>(bits)) continue;
+              const float v = HALF ? __half2float(__ushort_as_half(bits)) : __uint_as_float((uint32_t)bits << 16);
+              if (key0 + key <= lim[0]) o[i][e] += v;
+              if (key0 + key <= lim[1]) o[i][2 + e] += v;
+            }
+        }
+        __syncwarp();
       }
     }
   }
@@ -338,7 +411,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) paged_rows_kernel(const __g
         dst[d + kCol * (2 * t + 1)] = o[i][2 * r + 1];
       }
       if (t == 0) {
-        part_m[warp * 16 + row] = m[r];
+        part_m[warp * 16 + row] = m[r] + lv;
         part_l[warp * 16 + row] = l[r];
       }
     }
