@@ -2,7 +2,7 @@
 //
 // The work is reading the cache once: 16 rows of arithmetic ride on every key, so the kernel is bound by HBM, and with one
 // short sequence by latency. A work item is (16 rows, key head): the rows are consecutive tokens times the query heads that
-// share the key head. Its keys are split over the CTAs of a cluster and their four warps, 16 keys at a time.
+// share the key head. Its keys are split over the CTAs of a cluster and their warps, 16 or 32 keys at a time.
 //   copies   each lane copies its own fragments into its own slots of shared memory with cp.async, several blocks ahead, and
 //            reads them back itself: no barrier, and the copies in flight cost no registers. A key that nobody sees (behind
 //            the context, no page) is filled with zeros, so that nothing stale meets a probability of zero.
@@ -20,21 +20,28 @@
 
 namespace pgb {
 
-constexpr int kRowWarps = 4;
-
 template <int D, bool I8>
 struct RowTile {
+  // Warps that share an item's keys. Short rows: two, so that all the items of a batch run at once (64 sequences, 12 heads of
+  // 64: 37 us against 41 with four); long ones: four (16 sequences of up to 32768 int8 tokens, 8 heads of 128: 184 us
+  // against 191 with two and 254 with eight).
+  static constexpr int kWarps = D == 64 ? 2 : 4;
+  static constexpr int kCtas = 12 / kWarps;  // resident on an SM, as registers allow
   static constexpr int kEs = I8 ? 1 : 2;
   static constexpr int kKChunks = D * kEs / 64;              // 16-byte chunks of one key that a lane holds
   static constexpr int kVBytes = D * kEs / 8;                // bytes of one value row that a lane holds
   static constexpr int kVPiece = kVBytes < 16 ? 8 : 16;      // copied at once
   static constexpr int kVPieces = kVBytes / kVPiece;
   static constexpr int kK = 2 * kKChunks * 512, kV = 4 * kVPieces * 32 * kVPiece;
-  static constexpr int kStage = kK + kV + (I8 ? 128 : 0);    // 16 keys of one warp; an int8 block carries its 32 scales
-  static constexpr int kStages = D * kEs > 128 ? 3 : (D * kEs == 128 ? 4 : 6);
+  static constexpr int kSub = kK + kV + (I8 ? 128 : 0);      // 16 keys of one warp; with int8 their 32 scales
+  // Sub-blocks a warp takes at once: with short rows two, whose chains of products overlap and which share one turn of the
+  // running maximum (64 sequences of 1024, 12 heads of 64: 43 us with one).
+  static constexpr int kSubs = D == 64 ? 2 : 1;
+  static constexpr int kStage = kSubs * kSub;
+  static constexpr int kStages = kEs * kSubs == 4 ? 2 : (D * kEs > 128 || kSubs == 2 ? 3 : 4);
   static constexpr int kWarp = kStages * kStage;
-  static constexpr int kJoin = kRowWarps * 16 * (D + 2) * 4;
-  static constexpr int kSmem = (kRowWarps * kWarp > kJoin ? kRowWarps * kWarp : kJoin) + 16 * (D + 2) * 4;
+  static constexpr int kJoin = kWarps * 16 * (D + 2) * 4;
+  static constexpr int kSmem = (kWarps * kWarp > kJoin ? kWarps * kWarp : kJoin) + 16 * (D + 2) * 4;
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
@@ -86,9 +93,10 @@ __device__ __forceinline__ void cluster_sync() {
 }
 
 template <bool HALF, int D, bool I8>
-__global__ void __launch_bounds__(kRowWarps * 32, 3) paged_rows_kernel(const __grid_constant__ PagedParams a, const __grid_constant__ KvCache c,
+__global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::kCtas) paged_rows_kernel(const __grid_constant__ PagedParams a, const __grid_constant__ KvCache c,
                                                                        const __grid_constant__ KvPlan p, unsigned splits, unsigned tiles_per_token) {
   using S = RowTile<D, I8>;
+  constexpr int kRowWarps = S::kWarps;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, t = lane & 3;
   const int rank = (int)(blockIdx.x % splits);  // of the CTA in its cluster
@@ -109,7 +117,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) paged_rows_kernel(const __g
   const int held = p.width << c.log2_page;  // at most 2^30
   const int pos0 = (int)max(kv_position(p, seq, row0), -((int64_t)1 << 31));
   const int n_keys = max(0, min(held, pos0 + n_tok));  // what the tile's last token sees
-  const int n_blocks = (n_keys + 15) >> 4;
+  const int n_blocks = (n_keys + 16 * S::kSubs - 1) / (16 * S::kSubs);
 
   // Q in the order in which the chunks of K arrive: value i of this lane's D / 4 is d = 16/es * (t + 4 (i es / 16)) + ...
   // Beside an int8 cache the products run in fp16: there a key widens in fewer steps than in bf16. A bf16 row of Q is brought
@@ -165,15 +173,23 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) paged_rows_kernel(const __g
   const int *table = p.table + (int64_t)seq * p.pitch;
   const uint8_t *k_head = c.k.base + kvh * c.k.head + quad * c.k.slot + t * 16, *v_head = c.v.base + kvh * c.v.head + 2 * t * c.v.slot + quad * S::kVPiece;
   // the table's entry for block kb; looked up long before it is judged
-  auto entry_of = [&](int kb) -> int { return kb < n_blocks ? __ldg(table + (kb >> (c.log2_page - 4))) : -1; };
-  // Starts the copies of block kb (of the page given) into a stage. What the lane copies is what it reads.
-  auto fetch = [&](int kb, int page, int stage) {
-    if (kb < n_blocks) {
-      const uint32_t dst = base + stage * S::kStage;
-      const int slot0 = (kb << 4) & page_mask;
+  struct Entries { int page[S::kSubs]; };
+  auto entry_of = [&](int kb) -> Entries {
+    Entries e;
+#pragma unroll
+    for (int u = 0; u < S::kSubs; ++u) {
+      const int key0 = (kb * S::kSubs + u) << 4;
+      e.page[u] = key0 < n_keys ? __ldg(table + (key0 >> c.log2_page)) : -1;
+    }
+    return e;
+  };
+  // Starts the copies of 16 keys (of the page given) into their place. What the lane copies is what it reads.
+  auto fetch_sub = [&](int key0, int page, uint32_t dst) {
+    {
+      const int slot0 = key0 & page_mask;
       const bool ok = (unsigned)page < (unsigned)c.n_pages;
       const int64_t pg = ok ? page : 0;
-      const int there = ok ? n_keys - (kb << 4) : 0;  // keys of the block that exist, if fewer than 16
+      const int there = ok ? n_keys - key0 : 0;  // keys that exist, if fewer than 16
       const uint8_t *k = k_head + pg * c.k.page + slot0 * c.k.slot, *v = v_head + pg * c.v.page + slot0 * c.v.slot;
       auto pieces = [&](auto whole) {
         constexpr bool kWhole = decltype(whole)::value;
@@ -204,6 +220,12 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) paged_rows_kernel(const __g
         copy16(dst + S::kK + S::kV + lane * 16, s, ok);
       }
     }
+  };
+  auto fetch = [&](int kb, const Entries &e, int stage) {
+    if (kb < n_blocks) {
+#pragma unroll
+      for (int u = 0; u < S::kSubs; ++u) fetch_sub((kb * S::kSubs + u) << 4, e.page[u], base + stage * S::kStage + u * S::kSub);
+    }
     copy_commit();  // empty groups keep the count
   };
 
@@ -214,14 +236,19 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) paged_rows_kernel(const __g
   // stay within fp16, and since it is the same for all rows and in the sums too, O / l is what it was.
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, lv = I8 ? -100.f : 0.f;
 
-  int pages[S::kStages];  // table entries of the blocks under way
+  Entries pages[S::kStages];  // table entries of the blocks under way
 #pragma unroll
   for (int i = 0; i < S::kStages; ++i) pages[i] = entry_of(block0 + i * step);
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) fetch(block0 + i * step, pages[i], i);
   int stage = 0;
   for (int kb = block0; kb < n_blocks; kb += step) {
-    const bool absent = (unsigned)pages[0] >= (unsigned)c.n_pages;
+    bool absent[S::kSubs], any_absent = false;
+#pragma unroll
+    for (int u = 0; u < S::kSubs; ++u) {
+      absent[u] = (unsigned)pages[0].page[u] >= (unsigned)c.n_pages;
+      any_absent |= absent[u];
+    }
     fetch(kb + (S::kStages - 1) * step, pages[S::kStages - 1], stage == 0 ? S::kStages - 1 : stage - 1);
 #pragma unroll
     for (int i = 0; i + 1 < S::kStages; ++i) pages[i] = pages[i + 1];
@@ -231,60 +258,67 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) paged_rows_kernel(const __g
     const uint32_t src = base + stage * S::kStage;
     stage = stage + 1 == S::kStages ? 0 : stage + 1;
 
-    float s[2][4] = {};  // keys quad-wise: [h][0..1] row quad, [h][2..3] row quad + 8; keys 2t, 2t + 1 of half h
+    constexpr int U = S::kSubs;
+    float s[U][2][4] = {};  // of sub-block u, half h: [0..1] row quad, [2..3] row quad + 8; keys 2t, 2t + 1 of the half
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int j = 0; j < S::kKChunks; ++j)
 #pragma unroll
-      for (int j = 0; j < S::kKChunks; ++j) {
-        const uint4 r = ld_shared16(src + ((h * S::kKChunks + j) * 32 + lane) * 16);
-        if constexpr (I8) {
-          const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mma16816<true>(s[h], q[4 * j + e], paged_widen2<true>(w[e], 0), paged_widen2<true>(w[e], 1));
-        } else {
-          mma16816<HALF>(s[h], q[2 * j], r.x, r.y);
-          mma16816<HALF>(s[h], q[2 * j + 1], r.z, r.w);
+        for (int h = 0; h < 2; ++h) {
+          const uint4 r = ld_shared16(src + u * S::kSub + ((h * S::kKChunks + j) * 32 + lane) * 16);
+          if constexpr (I8) {
+            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mma16816<true>(s[u][h], q[4 * j + e], paged_widen2<true>(w[e], 0), paged_widen2<true>(w[e], 1));
+          } else {
+            mma16816<HALF>(s[u][h], q[2 * j], r.x, r.y);
+            mma16816<HALF>(s[u][h], q[2 * j + 1], r.z, r.w);
+          }
         }
+    const int key0 = kb * (16 * U);
+    const bool masked = key0 + 16 * U - 1 > lim_min || any_absent;  // warp-uniform
+    float vs[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if constexpr (I8) {
+        const uint32_t at = src + u * S::kSub + S::kK + S::kV + 8 * t;
+        const uint2 k0 = ld_shared8(at), k1 = ld_shared8(at + 32), v0 = ld_shared8(at + 64), v1 = ld_shared8(at + 96);
+        const float ks[4] = {__uint_as_float(k0.x), __uint_as_float(k0.y), __uint_as_float(k1.x), __uint_as_float(k1.y)};
+        vs[u][0] = __uint_as_float(v0.x); vs[u][1] = __uint_as_float(v0.y); vs[u][2] = __uint_as_float(v1.x); vs[u][3] = __uint_as_float(v1.y);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[u][h][e] *= ks[2 * h + (e & 1)];
       }
-    }
-    const int key0 = kb << 4;
-    const bool masked = key0 + 15 > lim_min || absent;  // warp-uniform
-    float vs[4];
-    if constexpr (I8) {
-      const uint32_t at = src + S::kK + S::kV + 8 * t;
-      const uint2 k0 = ld_shared8(at), k1 = ld_shared8(at + 32), v0 = ld_shared8(at + 64), v1 = ld_shared8(at + 96);
-      const float ks[4] = {__uint_as_float(k0.x), __uint_as_float(k0.y), __uint_as_float(k1.x), __uint_as_float(k1.y)};
-      vs[0] = __uint_as_float(v0.x); vs[1] = __uint_as_float(v0.y); vs[2] = __uint_as_float(v1.x); vs[3] = __uint_as_float(v1.y);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[h][e] *= ks[2 * h + (e & 1)];
-    }
+        for (int e = 0; e < 4; ++e) s[u][h][e] *= scale[e >> 1];
+      if (masked) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[h][e] *= scale[e >> 1];
-    if (masked) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = key0 + 8 * h + 2 * t + (e & 1);
-          if (key > lim[e >> 1] || absent) s[h][e] = -INFINITY;
-          // a slot behind the context has a stale scale: its probability of zero must meet a number
-          if (I8 && e < 2 && (key >= n_keys || absent)) vs[2 * h + e] = 0.f;
-        }
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + 16 * u + 8 * h + 2 * t + (e & 1);
+            if (key > lim[e >> 1] || absent[u]) s[u][h][e] = -INFINITY;
+            // a slot behind the context has a stale scale: its probability of zero must meet a number
+            if (I8 && e < 2 && (key >= n_keys || absent[u])) vs[u][2 * h + e] = 0.f;
+          }
+      }
     }
     float mx[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      mx[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+      mx[r] = fmaxf(fmaxf(s[0][0][2 * r], s[0][0][2 * r + 1]), fmaxf(s[0][1][2 * r], s[0][1][2 * r + 1]));
+      if (U == 2) mx[r] = fmaxf(mx[r], fmaxf(fmaxf(s[U - 1][0][2 * r], s[U - 1][0][2 * r + 1]), fmaxf(s[U - 1][1][2 * r], s[U - 1][1][2 * r + 1])));
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
     }
     float lv_new = lv;
     if constexpr (I8) {
-      float top = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+      float top = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[0][2], vs[0][3]));
+      if (U == 2) top = fmaxf(top, fmaxf(fmaxf(vs[U - 1][0], vs[U - 1][1]), fmaxf(vs[U - 1][2], vs[U - 1][3])));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const uint32_t e = __float_as_uint(top) >> 23;
@@ -307,73 +341,76 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) paged_rows_kernel(const __g
       }
     }
     const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0] + lv, m[1] == -INFINITY ? 0.f : m[1] + lv};
-    // The probabilities as the A operand of the second product: the accumulator's layout is the operand's.
-    uint32_t pa[4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float x = paged_ex2(s[h][2 * r] - ref[r]), y = paged_ex2(s[h][2 * r + 1] - ref[r]);
-        l[r] += x + y;
-        if (I8) {  // a token that a row does not see may have a scale that is no number
-          x = x == 0.f ? 0.f : x * vs[2 * h];
-          y = y == 0.f ? 0.f : y * vs[2 * h + 1];
-        }
-        pa[2 * h + r] = paged_pack<kHalfMma>(x, y);
-      }
-    const uint32_t vsrc = src + S::kK + lane * S::kVPiece;
     bool cleared = false;
-    auto value_words = [&](int g, int j) -> uint4 {
-      const uint32_t at = vsrc + (g * S::kVPieces + j) * 32 * S::kVPiece;
-      if constexpr (S::kVPiece == 16) {
-        uint4 r = ld_shared16(at);
-        // A new token that some rows must not see: NaN and infinities would reach them through a probability of zero.
-        if (!I8 && masked && key0 + 2 * t + (g & 1) + 8 * (g >> 1) > lim_min) {
-          uint32_t *w = reinterpret_cast<uint32_t *>(&r);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const bool lo = not_finite<HALF>(w[e] & 0xffffu), hi = not_finite<HALF>(w[e] >> 16);
-            if (lo) w[e] &= 0xffff0000u;
-            if (hi) w[e] &= 0xffffu;
-            cleared |= lo || hi;
+    for (int u = 0; u < U; ++u) {
+      // The probabilities as the A operand of the second product: the accumulator's layout is the operand's.
+      uint32_t pa[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float x = paged_ex2(s[u][h][2 * r] - ref[r]), y = paged_ex2(s[u][h][2 * r + 1] - ref[r]);
+          l[r] += x + y;
+          if (I8) {  // a token that a row does not see may have a scale that is no number
+            x = x == 0.f ? 0.f : x * vs[u][2 * h];
+            y = y == 0.f ? 0.f : y * vs[u][2 * h + 1];
           }
+          pa[2 * h + r] = paged_pack<kHalfMma>(x, y);
         }
-        return r;
-      } else {
-        const uint2 r = ld_shared8(at);
-        return make_uint4(r.x, r.y, 0, 0);
-      }
-    };
+      const uint32_t vsrc = src + u * S::kSub + S::kK + lane * S::kVPiece;
+      auto value_words = [&](int g, int j) -> uint4 {
+        const uint32_t at = vsrc + (g * S::kVPieces + j) * 32 * S::kVPiece;
+        if constexpr (S::kVPiece == 16) {
+          uint4 r = ld_shared16(at);
+          // A new token that some rows must not see: NaN and infinities would reach them through a probability of zero.
+          if (!I8 && masked && key0 + 16 * u + 2 * t + (g & 1) + 8 * (g >> 1) > lim_min) {
+            uint32_t *w = reinterpret_cast<uint32_t *>(&r);
 #pragma unroll
-    for (int j = 0; j < S::kVPieces; ++j) {
-      const uint4 r0 = value_words(0, j), r1 = value_words(1, j), r2 = value_words(2, j), r3 = value_words(3, j);
-      const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w}, w2[4] = {r2.x, r2.y, r2.z, r2.w}, w3[4] = {r3.x, r3.y, r3.z, r3.w};
-      constexpr int kWords = S::kVPiece / 4;
-#pragma unroll
-      for (int e = 0; e < kWords; ++e) {
-        if constexpr (I8) {
-          // bytes of two keys interleaved, then each pair widened: value d of keys 2t and 2t + 1 in one register
-          const uint32_t lo01 = __byte_perm(w0[e], w1[e], 0x5140), hi01 = __byte_perm(w0[e], w1[e], 0x7362);
-          const uint32_t lo23 = __byte_perm(w2[e], w3[e], 0x5140), hi23 = __byte_perm(w2[e], w3[e], 0x7362);
-#pragma unroll
-          for (int d = 0; d < 4; ++d)
-            mma16816<true>(o[j * kWords * 4 + 4 * e + d], pa, paged_widen2<true>(d < 2 ? lo01 : hi01, d & 1), paged_widen2<true>(d < 2 ? lo23 : hi23, d & 1));
+            for (int e = 0; e < 4; ++e) {
+              const bool lo = not_finite<HALF>(w[e] & 0xffffu), hi = not_finite<HALF>(w[e] >> 16);
+              if (lo) w[e] &= 0xffff0000u;
+              if (hi) w[e] &= 0xffffu;
+              cleared |= lo || hi;
+            }
+          }
+          return r;
         } else {
-          mma16816<HALF>(o[j * 8 + 2 * e], pa, __byte_perm(w0[e], w1[e], 0x5410), __byte_perm(w2[e], w3[e], 0x5410));
-          mma16816<HALF>(o[j * 8 + 2 * e + 1], pa, __byte_perm(w0[e], w1[e], 0x7632), __byte_perm(w2[e], w3[e], 0x7632));
+          const uint2 r = ld_shared8(at);
+          return make_uint4(r.x, r.y, 0, 0);
+        }
+      };
+#pragma unroll
+      for (int j = 0; j < S::kVPieces; ++j) {
+        const uint4 r0 = value_words(0, j), r1 = value_words(1, j), r2 = value_words(2, j), r3 = value_words(3, j);
+        const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w}, w2[4] = {r2.x, r2.y, r2.z, r2.w}, w3[4] = {r3.x, r3.y, r3.z, r3.w};
+        constexpr int kWords = S::kVPiece / 4;
+#pragma unroll
+        for (int e = 0; e < kWords; ++e) {
+          if constexpr (I8) {
+            // bytes of two keys interleaved, then each pair widened: value d of keys 2t and 2t + 1 in one register
+            const uint32_t lo01 = __byte_perm(w0[e], w1[e], 0x5140), hi01 = __byte_perm(w0[e], w1[e], 0x7362);
+            const uint32_t lo23 = __byte_perm(w2[e], w3[e], 0x5140), hi23 = __byte_perm(w2[e], w3[e], 0x7362);
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+              mma16816<true>(o[j * kWords * 4 + 4 * e + d], pa, paged_widen2<true>(d < 2 ? lo01 : hi01, d & 1), paged_widen2<true>(d < 2 ? lo23 : hi23, d & 1));
+          } else {
+            mma16816<HALF>(o[j * 8 + 2 * e], pa, __byte_perm(w0[e], w1[e], 0x5410), __byte_perm(w2[e], w3[e], 0x5410));
+            mma16816<HALF>(o[j * 8 + 2 * e + 1], pa, __byte_perm(w0[e], w1[e], 0x7632), __byte_perm(w2[e], w3[e], 0x7632));
+          }
         }
       }
     }
     if constexpr (!I8) {
       if (masked && __any_sync(0xffffffffu, cleared)) {  // rare: give back what was cleared, to the rows that see it
         __syncwarp();                                    // the values lie in other lanes' slots
-        for (int key = max(0, lim_min + 1 - key0); key < min(16, n_keys - key0); ++key) {
-          const int g = (key & 1) + 2 * (key >> 3), owner = (key & 7) >> 1;
+        for (int key = max(0, lim_min + 1 - key0); key < min(16 * U, n_keys - key0); ++key) {
+          const int g = (key & 1) + 2 * ((key >> 3) & 1), owner = (key & 7) >> 1;
 #pragma unroll
           for (int i = 0; i < D / 8; ++i)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const uint32_t at = src + S::kK + ((g * S::kVPieces + i / 8) * 32 + (2 * t + e) * 4 + owner) * 16 + 2 * (i % 8);
+              const uint32_t at = src + (key >> 4) * S::kSub + S::kK + ((g * S::kVPieces + i / 8) * 32 + (2 * t + e) * 4 + owner) * 16 + 2 * (i % 8);
               unsigned short bits;
               asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(at) : "memory");
               if (!not_finite<HALF>(bits)) continue;
@@ -484,7 +521,7 @@ static int launch(const PagedParams &a, const KvCache &c, const KvPlan &p, int s
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * splits));
-  cfg.blockDim = dim3(kRowWarps * 32);
+  cfg.blockDim = dim3(S::kWarps * 32);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -508,8 +545,9 @@ int run_paged_rows(const PagedParams &a, const KvCache &c, const KvPlan &p, bool
   const int64_t units = a.rows * tiles_per_token * c.heads;
   // As many CTAs per item as leave no SM idle, up to a portable cluster; not more than have a block of keys for each warp.
   int splits = 1;
-  const int64_t blocks = ((int64_t)p.width << c.log2_page) / 16;
-  while (splits < 8 && units * splits < 4LL * sm_count() && blocks > (int64_t)splits * kRowWarps) splits *= 2;
+  const int warps = c.head_dim == 64 ? 2 : 4;
+  const int64_t blocks = ((int64_t)p.width << c.log2_page) / (c.head_dim == 64 ? 32 : 16);
+  while (splits < 8 && units * splits < 4LL * sm_count() && blocks > (int64_t)splits * warps) splits *= 2;
   if (units * splits > 2147483647LL) {
     set_error("paged_attention: too many rows for one launch");
     return PGB_ERR_UNSUPPORTED;

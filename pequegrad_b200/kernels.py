@@ -270,33 +270,36 @@ def gemm_wait_drill(polls: int, skip_loads: bool = True) -> None:
 
 # ---- generation: the paged cache, attention over it, logits -----------------------------------------------------------
 
+_DTYPE_SIZE = {dt: (code, torch.empty((), dtype=dt).element_size()) for dt, code in _TORCH2PGB.items()}
+
+
 def _packed(ref: torch.Tensor, tensors) -> list:
     """Descriptors of tensors (None stays None) that must lie on `ref`'s device."""
-    out = []
-    dev = ref.device
-    if dev.type != "cuda":
+    dev = ref.get_device()
+    if not ref.is_cuda:
         raise RuntimeError("pgb200 kernels need CUDA tensors: there is no CPU path")
+    out = []
     for t in tensors:
         if t is None:
             out.append(None)
             continue
-        if t.device != dev:
-            raise ValueError(f"all tensors must be on one device: {t.device} and {dev}")
-        dt = _TORCH2PGB.get(t.dtype)
-        if dt is None:
+        if t.get_device() != dev:
+            raise ValueError(f"all tensors must be on one device: {t.device} and {ref.device}")
+        if t.dtype not in _DTYPE_SIZE:
             pgb_dtype(t.dtype)  # raises
-        es = t.element_size()
-        out.append(L.pack_tensor(t.data_ptr(), dt, t.shape, [s * es for s in t.stride()]))
+        code, size = _DTYPE_SIZE[t.dtype]
+        out.append(L.pack_tensor(t.data_ptr(), code, t.shape, [s * size for s in t.stride()]))
     return out
 
 
-def _call(fn, dev: torch.device, args) -> None:
+def _call(fn, dev: int, args) -> None:
     """fn(*args, the device's current stream) with that device current."""
-    if dev.index == torch.cuda.current_device():
-        st = fn(*args, torch.cuda.current_stream().cuda_stream)
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if dev == torch._C._cuda_getDevice():
+        st = fn(*args, stream)
     else:
         with torch.cuda.device(dev):
-            st = fn(*args, torch.cuda.current_stream().cuda_stream)
+            st = fn(*args, stream)
     if st != L.OK:
         L.check(st)
 
@@ -306,7 +309,7 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     """Store new rows k, v [rows, heads, D] in a paged cache [pages, heads, page size, D]: a copy, or int8 with one scale per
     token and head (k_scale / v_scale [pages, heads, page size] float32). q_start [B + 1], ctx_len [B] (new tokens included)
     and page_table [B, n] are int32 on the device; a position whose table entry is no page is not stored."""
-    _call(L.lib().pgb_kv_write, k.device, _packed(k, (k, v, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len, page_table)))
+    _call(L.lib().pgb_kv_write, k.get_device(), _packed(k, (k, v, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len, page_table)))
 
 
 def kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_start: torch.Tensor, page_table: torch.Tensor, rows: int,
@@ -320,7 +323,7 @@ def kv_read(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_start: torch.Tensor
         out = torch.empty(shape, dtype=dt, device=k_cache.device), torch.empty(shape, dtype=dt, device=k_cache.device)
     elif out[0].shape[0] != rows or (out_dtype is not None and out[0].dtype != out_dtype):
         raise ValueError("kv_read: out does not have the rows or the dtype asked for")
-    _call(L.lib().pgb_kv_read, k_cache.device, _packed(k_cache, (k_cache, v_cache, k_scale, v_scale, kv_start, page_table, *out)))
+    _call(L.lib().pgb_kv_read, k_cache.get_device(), _packed(k_cache, (k_cache, v_cache, k_scale, v_scale, kv_start, page_table, *out)))
     return out
 
 
@@ -336,7 +339,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     a = _packed(q, (q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len, page_table, out))
     a.insert(8, scale)
-    _call(L.lib().pgb_paged_attention, q.device, a)
+    _call(L.lib().pgb_paged_attention, q.get_device(), a)
     return out
 
 
@@ -348,7 +351,7 @@ def logits_process(logits: torch.Tensor, history: torch.Tensor | None = None, hi
     is clear set to -inf (the formula stands at pgb_logits_process). `out` may be `logits`."""
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    _call(L.lib().pgb_logits_process, logits.device,
+    _call(L.lib().pgb_logits_process, logits.get_device(),
           _packed(logits, (logits, history, history_len, prompt_len, repetition, frequency, presence, bias_ids, bias, mask, out)))
     return out
 
