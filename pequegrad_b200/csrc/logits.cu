@@ -9,6 +9,7 @@
 // The work is one read and one write of the logits; the counts never leave the SM: a CTA owns a slice of one row's
 // vocabulary, counts the history's tokens that fall into it with integer atomics in shared memory (their order does not
 // change the result), and then streams its slice. Every CTA of a row reads the whole history, which the L2 serves.
+#include <cstring>
 #include <string>
 
 #include "reduce_common.cuh"
@@ -17,6 +18,10 @@
 namespace pgb {
 
 constexpr int kLogitThreads = 256;
+// Vocabulary entries per CTA: two 16-byte vectors a thread.
+template <typename IoT> constexpr int kLogitSlice = 2 * kLogitThreads * 16 / (int)sizeof(IoT);
+// A shared-memory array of them, with room to shift them as a row's start requires.
+template <typename IoT> constexpr int kLogitRoom = kLogitSlice<IoT> + 8;
 constexpr uint32_t kSeen = 0x80000000u;  // bit 31 of a counter: the token occurs at all; the rest counts the generated ones
 
 struct LogitParams {
@@ -34,48 +39,92 @@ struct LogitParams {
   int n_bias;
   const uint32_t *mask;
   int64_t mask_pitch;  // words
-  int slice;           // vocabulary entries per CTA
 };
+
+// V consecutive values as they lie in memory
+template <typename IoT, int V>
+struct alignas(sizeof(IoT) * V) RawVec { IoT v[V]; };
 
 template <typename IoT, int V>
 __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const __grid_constant__ LogitParams p) {
-  extern __shared__ uint32_t smem[];
+  constexpr int kSlice = kLogitSlice<IoT>, kArray = kLogitRoom<IoT>, kVecs = kSlice / (kLogitThreads * V);
+  extern __shared__ __align__(16) uint32_t smem[];
   const int64_t row = blockIdx.y;
-  const int64_t v0 = (int64_t)blockIdx.x * p.slice;
-  const int n = (int)min((int64_t)p.slice, p.V - v0);
+  const int64_t v0 = (int64_t)blockIdx.x * kSlice;
+  const int n = (int)min((int64_t)kSlice, p.V - v0);
   const bool counts = p.history != nullptr, biased = p.n_bias > 0;
   uint32_t *count = smem;
-  float *bias = reinterpret_cast<float *>(smem + (counts ? p.slice : 0));
-  if (counts)
-    for (int i = threadIdx.x; i < n; i += kLogitThreads) count[i] = 0;
-  if (biased)
-    for (int i = threadIdx.x; i < n; i += kLogitThreads) bias[i] = 0.f;
+  float *bias = reinterpret_cast<float *>(smem + (counts ? kArray : 0));
+  // where x and y are not aligned alike, the results pass through shared memory
+  IoT *staged = reinterpret_cast<IoT *>(smem + (counts + biased) * kArray);
+  const IoT *x = (const IoT *)p.x + row * p.x_pitch + v0;
+  IoT *y = (IoT *)p.y + row * p.y_pitch + v0;
+  // Rows start anywhere (50257 halves in a row: at any even address). Whole 16-byte vectors of x are taken, from entry `first`
+  // on; the few entries before and behind them one by one. The arrays in shared memory are shifted likewise, so that a
+  // vector's counts and biases are whole vectors too.
+  const int shift = (int)((reinterpret_cast<uintptr_t>(x) / sizeof(IoT)) % V), first = (V - shift) % V;
+  const int n_vec = max(0, n - first) / V;
+  count += shift;
+  bias += shift;
+  // the slice is on its way while the history is counted
+  RawVec<IoT, V> raw[kVecs];
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    const int k = u * kLogitThreads + threadIdx.x;
+    if (k < n_vec) {
+      const uint4 r = __ldcs(reinterpret_cast<const uint4 *>(x + first + k * V));
+      memcpy(&raw[u], &r, 16);
+    }
+  }
+  // The last warp takes the biases, where there are any, the others the history. Its first tokens are fetched before its
+  // length is known: what lies behind the length is not used.
+  const int counters = kLogitThreads - (biased ? 32 : 0);
+  const int *h = p.history + row * p.history_pitch;
+  int len = 0, prompt = 0, early[4] = {};
+  if (counts && threadIdx.x < counters) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if ((int)threadIdx.x + u * counters < p.L) early[u] = __ldg(h + threadIdx.x + u * counters);
+    len = p.history_len ? min(max(__ldg(p.history_len + row), 0), p.L) : p.L;
+    prompt = p.prompt_len ? __ldg(p.prompt_len + row) : 0;
+  }
+  for (int i = threadIdx.x * 4; i < (counts + biased) * kArray; i += kLogitThreads * 4) *reinterpret_cast<uint4 *>(smem + i) = make_uint4(0, 0, 0, 0);
   __syncthreads();
-  if (counts) {
-    const int len = p.history_len ? min(max(__ldg(p.history_len + row), 0), p.L) : p.L;
-    const int prompt = p.prompt_len ? __ldg(p.prompt_len + row) : 0;
-    const int *h = p.history + row * p.history_pitch;
-    for (int i = threadIdx.x; i < len; i += kLogitThreads) {
-      const int64_t at = (int64_t)__ldg(h + i) - v0;
-      if (at < 0 || at >= n) continue;
+  if (counts && threadIdx.x < counters) {
+    auto put = [&](int i, int id) {
+      const int64_t at = (int64_t)id - v0;
+      if (at < 0 || at >= n) return;
       if (i >= prompt) {
         if ((atomicAdd(count + at, 1u) & kSeen) == 0) atomicOr(count + at, kSeen);
       } else {
         atomicOr(count + at, kSeen);
       }
+    };
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if ((int)threadIdx.x + u * counters < len) put(threadIdx.x + u * counters, early[u]);
+    int i = threadIdx.x + 4 * counters;
+    for (; i + 3 * counters < len; i += 4 * counters) {  // four loads under way
+      const int a = __ldg(h + i), b = __ldg(h + i + counters), c = __ldg(h + i + 2 * counters), d = __ldg(h + i + 3 * counters);
+      put(i, a);
+      put(i + counters, b);
+      put(i + 2 * counters, c);
+      put(i + 3 * counters, d);
     }
+    for (; i < len; i += counters) put(i, __ldg(h + i));
   }
   // A token may be biased more than once. One warp takes the list in order, and lanes that hold the same token leave the
   // sum to the first of them, which adds in list order: the result does not depend on timing.
-  if (biased && threadIdx.x < 32) {
+  if (biased && threadIdx.x >= counters) {
     const int *ids = p.bias_ids + row * p.bias_ids_pitch;
     const float *val = p.bias + row * p.bias_pitch;
-    const int lane = threadIdx.x;
+    const int lane = threadIdx.x & 31;
     for (int i0 = 0; i0 < p.n_bias; i0 += 32) {
       const bool in = i0 + lane < p.n_bias;
       const int64_t at = in ? (int64_t)__ldg(ids + i0 + lane) - v0 : -1;
       const float b = in ? __ldg(val + i0 + lane) : 0.f;
       const bool mine = at >= 0 && at < n;
+      if (!__any_sync(0xffffffffu, mine)) continue;
       const uint32_t same = __match_any_sync(0xffffffffu, mine ? (int)at : -1);
       const bool first = mine && (__ffs(same) - 1) == lane;
       float sum = first ? bias[at] + b : 0.f;
@@ -94,35 +143,71 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const __grid_cons
   const float rep = p.repetition ? __ldg(p.repetition + row) : 1.f;
   const float freq = p.frequency ? __ldg(p.frequency + row) : 0.f;
   const float pres = p.presence ? __ldg(p.presence + row) : 0.f;
-  const IoT *x = (const IoT *)p.x + row * p.x_pitch + v0;
-  IoT *y = (IoT *)p.y + row * p.y_pitch + v0;
   const uint32_t *mask = p.mask ? p.mask + row * p.mask_pitch : nullptr;
-  auto shape = [&](float f, int i, uint32_t allowed) -> float {
-    if (counts) {
-      const uint32_t c = count[i];
-      if (c) {
-        f = f > 0.f ? f / rep : f * rep;
-        const uint32_t made = c & ~kSeen;
-        if (made) f = f - freq * (float)made - pres;
-      }
+  auto shape = [&](float f, uint32_t c, float b, uint32_t allowed) -> float {
+    if (c) {
+      f = f > 0.f ? f / rep : f * rep;
+      const uint32_t made = c & ~kSeen;
+      if (made) f = f - freq * (float)made - pres;
     }
-    if (biased) f = f + bias[i];
+    if (biased) f = f + b;
     return allowed ? f : -INFINITY;
   };
-  const int nv = n / V * V;
-  for (int i = threadIdx.x * V; i < nv; i += kLogitThreads * V) {
-    float f[V];
-    load_vec<float, IoT, V>(x + i, f);
-    const int64_t v = v0 + i;  // V entries share a mask word: V divides 32 and v is a multiple of V
-    const uint32_t bits = mask ? __ldg(mask + (v >> 5)) >> (v & 31) : 0xffffffffu;
+  // bit e of the result: may entry i + e follow
+  auto allowed = [&](int i) -> uint32_t {
+    if (!mask) return 0xffffffffu;
+    const int64_t v = v0 + i, w = v >> 5;
+    const uint32_t lo = __ldg(mask + w), hi = (v & 31) + V > 32 && (w + 1) * 32 < p.V ? __ldg(mask + w + 1) : 0u;
+    return __funnelshift_r(lo, hi, (uint32_t)(v & 31));
+  };
+  const int y_shift = (int)((reinterpret_cast<uintptr_t>(y) / sizeof(IoT)) % V);
+  const bool alike = y_shift == shift;
 #pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = shape(f[e], i + e, (bits >> e) & 1);
-    store_vec<IoT, float, V>(y + i, f);
+  for (int u = 0; u < kVecs; ++u) {
+    const int k = u * kLogitThreads + threadIdx.x;
+    if (k >= n_vec) continue;
+    const int i = first + k * V;
+    // counts and biases in 16-byte reads: word by word, eight lanes would meet in each bank
+    uint32_t c[V] = {};
+    float b[V] = {};
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      if (counts) {
+        const uint4 r = *reinterpret_cast<const uint4 *>(count + i + e);
+        c[e] = r.x; c[e + 1] = r.y; c[e + 2] = r.z; c[e + 3] = r.w;
+      }
+      if (biased) {
+        const float4 r = *reinterpret_cast<const float4 *>(bias + i + e);
+        b[e] = r.x; b[e + 1] = r.y; b[e + 2] = r.z; b[e + 3] = r.w;
+      }
+    }
+    const uint32_t bits = allowed(i);
+    float f[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = shape(to_compute<float, IoT>(raw[u].v[e]), c[e], b[e], (bits >> e) & 1);
+    if (alike) {
+      store_vec<IoT, float, V>(y + i, f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) staged[y_shift + i + e] = from_compute<IoT, float>(f[e]);
+    }
   }
-  for (int i = nv + threadIdx.x; i < n; i += kLogitThreads) {  // the ragged end of the row
-    const int64_t v = v0 + i;
-    const uint32_t bit = mask ? (__ldg(mask + (v >> 5)) >> (v & 31)) & 1 : 1u;
-    y[i] = from_compute<IoT, float>(shape(to_compute<float, IoT>(x[i]), i, bit));
+  // the entries before the first vector and behind the last
+  const int head = min(first, n), tail = first + n_vec * V, rest = head + max(0, n - tail);
+  if (threadIdx.x < rest) {
+    const int i = threadIdx.x < head ? threadIdx.x : tail + threadIdx.x - head;
+    const IoT f = from_compute<IoT, float>(shape(to_compute<float, IoT>(x[i]), counts ? count[i] : 0u, biased ? bias[i] : 0.f, allowed(i) & 1));
+    if (alike) y[i] = f;
+    else staged[y_shift + i] = f;
+  }
+  if (alike) return;
+  __syncthreads();
+  const int y_first = (V - y_shift) % V, y_vec = max(0, n - y_first) / V, y_tail = y_first + y_vec * V, y_head = min(y_first, n);
+  for (int k = threadIdx.x; k < y_vec; k += kLogitThreads)
+    *reinterpret_cast<uint4 *>(y + y_first + k * V) = *reinterpret_cast<const uint4 *>(staged + y_shift + y_first + k * V);
+  if (threadIdx.x < y_head + max(0, n - y_tail)) {
+    const int i = threadIdx.x < y_head ? threadIdx.x : y_tail + threadIdx.x - y_head;
+    y[i] = staged[y_shift + i];
   }
 }
 
@@ -203,19 +288,15 @@ static int logits_process(const pgb_tensor *logits, const pgb_tensor *history, c
   p.bias_ids = (const int *)ptr(bias_ids);
   p.bias = (const float *)ptr(bias);
   p.mask = (const uint32_t *)ptr(mask);
-  p.slice = 4096;
-  const dim3 grid((unsigned)((V + p.slice - 1) / p.slice), (unsigned)rows);
-  const size_t smem = ((p.history ? 1 : 0) + (p.n_bias ? 1 : 0)) * (size_t)p.slice * 4;
-  const bool aligned = !(reinterpret_cast<uintptr_t>(p.x) & 15) && !(reinterpret_cast<uintptr_t>(p.y) & 15) && (p.x_pitch * es) % 16 == 0 && (p.y_pitch * es) % 16 == 0;
-#define PGB_LOGITS(T, N)                                                  \
-  do {                                                                    \
-    if (aligned) logits_kernel<T, N><<<grid, kLogitThreads, smem, stream>>>(p); \
-    else logits_kernel<T, 1><<<grid, kLogitThreads, smem, stream>>>(p);         \
-  } while (0)
-  if (logits->dtype == PGB_F32) PGB_LOGITS(float, 4);
-  else if (logits->dtype == PGB_F16) PGB_LOGITS(__half, 8);
-  else PGB_LOGITS(__nv_bfloat16, 8);
-#undef PGB_LOGITS
+  // alike for every row where the bases are alike and the pitches differ by whole vectors, or there is one row
+  const bool alike = (reinterpret_cast<uintptr_t>(p.x) - reinterpret_cast<uintptr_t>(p.y)) % 16 == 0 && ((p.x_pitch - p.y_pitch) * es) % 16 == 0;
+  auto launch = [&](auto kernel, int slice, int room) {
+    const size_t smem = ((p.history ? 1 : 0) + (p.n_bias ? 1 : 0)) * (size_t)room * 4 + (alike ? 0 : (size_t)room * es);
+    kernel<<<dim3((unsigned)((V + slice - 1) / slice), (unsigned)rows), kLogitThreads, smem, stream>>>(p);
+  };
+  if (logits->dtype == PGB_F32) launch(logits_kernel<float, 4>, kLogitSlice<float>, kLogitRoom<float>);
+  else if (logits->dtype == PGB_F16) launch(logits_kernel<__half, 8>, kLogitSlice<__half>, kLogitRoom<__half>);
+  else launch(logits_kernel<__nv_bfloat16, 8>, kLogitSlice<__nv_bfloat16>, kLogitRoom<__nv_bfloat16>);
   count_launch();
   return check_launch("logits_kernel");
 }
