@@ -373,7 +373,7 @@ PGB_API int pgb_peer_allgather(const void *src, size_t bytes, void *const *peer_
                                int world, void *stream);
 
 /* ---- Generation: a paged key / value cache, attention over it, logits ------------------------------------------------
- * The reference's GPT-2 generates by recomputing every position for each new token (examples/gpt2.py:383-402); these
+ * The reference's GPT-2 generates by recomputing every position for each new token (examples/gpt2.py:406-438); these
  * entry points have no counterpart there.
  *
  * A cache is two tensors k_cache and v_cache [pages, heads, page size, head dim], f16, bf16 or int8: views with a

@@ -1,7 +1,7 @@
 // The paged key / value cache as the kernels see it: views of the pages, the plan that maps packed rows to sequences
 // and positions, and the host-side checks that the entry points of the cache share.
 //
-// The reference's GPT-2 recomputes every position for each new token (examples/gpt2.py:383-402) and has no cache.
+// The reference's GPT-2 recomputes every position for each new token (examples/gpt2.py:406-438) and has no cache.
 #pragma once
 #include <string>
 

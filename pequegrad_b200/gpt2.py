@@ -9,6 +9,11 @@ in every GEMM and in LayerNorm / softmax. Per layer the launches are:
   one kernel, heads read from and written to the packed [B, T, C] buffers) |
   proj GEMM(+bias,+residual) | layernorm | fc GEMM(+bias,+GELU) | proj GEMM(+bias,+residual)
 Weights of a Linear are kept transposed ([out, in], K-major for the GEMM).
+Generation keeps every token's keys and values in a paged cache (`kvcache`): `forward_cached` runs only the new
+tokens of some sequences (whole prompts, chunks of them, single tokens, mixed), per layer
+  layernorm | qkv GEMM(+bias) | store k, v | attention over the cache | proj GEMM | layernorm | fc GEMM | proj GEMM
+and `generate` picks tokens greedily (the reference's loop, examples/gpt2.py:406-438, runs the whole sequence again for
+each token), after penalties, biases and masks on the logits.
 `fused_attention=False` runs attention as the reference composes it (scores GEMM,
 causal softmax kernel, V transpose, PV GEMM) for comparison.
 """
@@ -17,7 +22,9 @@ from __future__ import annotations
 import numpy as np
 import torch
 
+from . import _lib as L
 from . import kernels as K
+from .kvcache import KVPlan, PagedKVCache
 
 
 class GPT2Config:
@@ -92,6 +99,96 @@ class GPT2:
         logits = logits_out[:, :, : cfg.vocab_size]
         K.matmul(x, self.lm_head_t.T, out=logits)
         return logits
+
+
+    # ---- generation ---------------------------------------------------------------------------------------------------
+
+    def new_cache(self, n_tokens: int, page_size: int = 16, dtype=None) -> PagedKVCache:
+        """A cache with room for `n_tokens` tokens in whole pages, in the model's dtype or in int8."""
+        cfg = self.cfg
+        return PagedKVCache(cfg.n_layer, cfg.n_head, cfg.n_embd // cfg.n_head, -(-n_tokens // page_size), page_size,
+                            self.dtype if dtype is None else dtype, self.wte.device)
+
+    def forward_cached(self, ids: torch.Tensor, cache: PagedKVCache, plan: KVPlan, last_only: bool = True) -> torch.Tensor:
+        """ids: the step's new tokens [plan.rows] int32, packed sequence after sequence. Returns the logits of each
+        sequence's last new token [sequences, vocab] (each must have one), or of every row."""
+        cfg = self.cfg
+        R, C, H = plan.rows, cfg.n_embd, cfg.n_head
+        D = C // H
+        if ids.shape != (R,):
+            raise ValueError("GPT2.forward_cached: one token id per row of the plan")
+        if plan.longest > cfg.block_size:
+            raise ValueError("GPT2.forward_cached: a sequence is longer than block_size")
+        tok, pos = K.embedding_rows(ids, self.wte, None, 1), K.embedding_rows(plan.positions, self.wpe, None, 1)
+        (x,) = K.fused_elementwise([tok, pos], [("LOAD", 0), ("LOAD", 1), ("ADD", 0, 1)])
+        for i, blk in enumerate(self.blocks):
+            h = K.layernorm_rows(x, blk["ln1_g"], blk["ln1_b"], 1e-5)
+            qkv = K.matmul(h, blk["attn_wt"].T, bias=blk["attn_b"]).view(R, 3, H, D)
+            cache.write(i, qkv[:, 1], qkv[:, 2], plan)
+            y = cache.attend(i, qkv[:, 0], plan, scale=float(D) ** -0.5).view(R, C)
+            x = K.matmul(y, blk["proj_wt"].T, bias=blk["proj_b"], residual=x)
+            h = K.layernorm_rows(x, blk["ln2_g"], blk["ln2_b"], 1e-5)
+            h = K.matmul(h, blk["fc_wt"].T, bias=blk["fc_b"], act=2)
+            x = K.matmul(h, blk["fc2_wt"].T, bias=blk["fc2_b"], residual=x)
+        if last_only:
+            x = K.embedding_rows(plan.last, x, None, 1)  # a gather of rows
+        x = K.layernorm_rows(x, self.lnf_g, self.lnf_b, 1e-5)
+        logits = torch.empty((x.shape[0], self.vocab_ld), dtype=self.dtype, device=x.device)[:, : cfg.vocab_size]
+        return K.matmul(x, self.lm_head_t.T, out=logits)
+
+    def generate(self, prompts, max_new: int, cache_dtype=None, page_size: int = 16, repetition: float = 1.0, frequency: float = 0.0,
+                 presence: float = 0.0, bias: dict | None = None, mask=None, eos: int | None = None) -> list:
+        """Greedy continuation of several prompts (lists of token ids) by up to `max_new` tokens each; a sequence ends behind
+        `eos`. Before each pick the logits are shaped (`kernels.logits_process`): tokens seen so far are divided by
+        `repetition`, generated ones lowered by `frequency` per occurrence and by `presence` once, `bias` {token: value} is
+        added, and `mask(tokens)`, called with the generated tokens of the sequences still running, gives the int32 bit mask
+        [sequences, words] of tokens that may follow, or None. Returns the generated tokens of each prompt."""
+        cfg, dev = self.cfg, self.wte.device
+        if max_new < 0 or any(len(p) == 0 or len(p) + max_new > cfg.block_size for p in prompts):
+            raise ValueError("GPT2.generate: prompts must not be empty, and with the new tokens not be longer than block_size")
+        if not prompts or max_new == 0:
+            return [[] for _ in prompts]
+        longest = max(len(p) for p in prompts) + max_new
+        cache = self.new_cache(sum(-(-(len(p) + max_new) // page_size) * page_size for p in prompts), page_size, cache_dtype)
+        seqs = [cache.open() for _ in prompts]
+        up = lambda a, dt: torch.tensor(a, dtype=dt).to(dev)  # noqa: E731
+        history = up([list(p) + [-1] * (longest - len(p)) for p in prompts], torch.int32)
+        prompt_len = up([len(p) for p in prompts], torch.int32)
+        out, live = [[] for _ in prompts], list(range(len(prompts)))
+        ids = up([t for p in prompts for t in p], torch.int32)
+        new = [len(p) for p in prompts]
+        for step in range(max_new):
+            plan = cache.extend([seqs[b] for b in live], new)
+            logits = self.forward_cached(ids, cache, plan)
+            n = len(live)
+            kw = {}
+            if repetition != 1.0 or frequency != 0.0 or presence != 0.0:
+                rows = history if n == len(prompts) else history[up(live, torch.int64)]
+                full = lambda v: torch.full((n,), v, dtype=torch.float32, device=dev)  # noqa: E731
+                kw.update(history=rows, history_len=plan.ctx_len, prompt_len=prompt_len if n == len(prompts) else prompt_len[up(live, torch.int64)],
+                          repetition=full(repetition), frequency=full(frequency), presence=full(presence))
+            if bias:
+                kw.update(bias_ids=up([list(bias)] * n, torch.int32), bias=up([list(bias.values())] * n, torch.float32))
+            if mask is not None:
+                kw["mask"] = mask([out[b] for b in live])
+            if kw:
+                K.logits_process(logits, out=logits, **kw)
+            tokens = K.fused_reduce([logits], L.ARGMAX, [1])
+            picked = tokens.tolist()
+            if repetition != 1.0 or frequency != 0.0 or presence != 0.0:
+                history[up(live, torch.int64), up([cache.length(seqs[b]) for b in live], torch.int64)] = tokens
+            for b, t in zip(live, picked):
+                out[b].append(t)
+            still = [i for i, b in enumerate(live) if eos is None or out[b][-1] != eos]
+            for b in live:
+                if eos is not None and out[b][-1] == eos:
+                    cache.close(seqs[b])
+            if not still:
+                break
+            ids = tokens if len(still) == n else tokens[up(still, torch.int64)]
+            live = [live[i] for i in still]
+            new = [1] * len(live)
+        return out
 
 
 def round_weights_fp16(weights: dict) -> dict:

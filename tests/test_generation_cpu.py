@@ -171,3 +171,57 @@ def test_logit_calls_that_are_refused():
     refused(logits(ids=f32(3, 2), bias=f32(3, 2)), bad, b"[rows, entries]")
     refused(logits(mask=i32(3, 3)), bad, b"a bit for each")
     refused(logits(mask=f32(3, 4)), bad, b"a bit for each")
+
+
+# ---- which sequence holds which page ------------------------------------------------------------------------------------
+
+def cache(pages, page_size=16, dtype=torch.float16):
+    from pequegrad_b200.kvcache import PagedKVCache
+    return PagedKVCache(2, 3, 64, pages, page_size, dtype, device="cpu")
+
+
+def test_plans_of_a_cache():
+    c = cache(8)
+    a, b = c.open(), c.open()
+    p = c.extend([a, b], [20, 16])
+    assert p.rows == 36 and p.longest == 20
+    assert p.q_start.tolist() == [0, 20, 36] and p.ctx_len.tolist() == [20, 16] and p.last.tolist() == [19, 35]
+    assert p.positions.tolist() == list(range(20)) + list(range(16))
+    assert p.page_table.shape == (2, 2) and p.page_table[1, 1] == -1
+    first = p.page_table[0].tolist()
+    used = set(first) | {int(p.page_table[1, 0])}
+    assert len(used) == 3 and c.free_pages() == 5
+    p = c.extend([b, a], [1, 1])  # in any order; b enters a new page, a does not
+    assert p.ctx_len.tolist() == [17, 21] and p.positions.tolist() == [16, 20] and p.last.tolist() == [0, 1]
+    assert p.page_table[1].tolist() == first and c.free_pages() == 4
+    assert not set(p.page_table[0].tolist()) & set(first)
+    c.close(b)
+    assert c.free_pages() == 6 and c.length(a) == 21
+    p = c.extend([a], [0])
+    assert p.rows == 0 and p.q_start.tolist() == [0, 0] and p.ctx_len.tolist() == [21]
+    assert c.extend([], []).page_table.shape == (0, 0)
+
+
+def test_a_cache_that_is_full_changes_nothing():
+    c = cache(3)
+    a, b = c.open(), c.open()
+    c.extend([a], [33])
+    with pytest.raises(RuntimeError, match="1 pages are needed and 0 are free"):
+        c.extend([a, b], [1, 1])
+    assert c.length(a) == 33 and c.length(b) == 0 and c.free_pages() == 0
+    c.extend([a], [15])
+    with pytest.raises(ValueError, match="each sequence once"):
+        c.extend([a, a], [1, 1])
+    with pytest.raises(ValueError, match="each sequence once"):
+        c.extend([a], [-1])
+    with pytest.raises(KeyError):
+        c.close(99)
+    c.close(a)
+    with pytest.raises(KeyError):
+        c.extend([a], [1])
+
+
+def test_an_int8_cache_has_scales_and_a_16_bit_cache_has_none():
+    assert cache(4).k_scale is None
+    c = cache(4, 32, torch.int8)
+    assert c.k.shape == (2, 4, 3, 32, 64) and c.v_scale.shape == (2, 4, 3, 32) and c.v_scale.dtype == torch.float32
