@@ -183,6 +183,12 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   memcpy(&d, &ud, 8);
   return d;
 }
+// maximum of three, NaN if one of them is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ void chunk_copy16(uint32_t dst, const void *src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
@@ -688,12 +694,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
           float mq[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            mq[q] = max3(__uint_as_float(x[8 * q]), __uint_as_float(x[8 * q + 1]), __uint_as_float(x[8 * q + 2]));
-            mq[q] = max3(mq[q], __uint_as_float(x[8 * q + 3]), __uint_as_float(x[8 * q + 4]));
-            mq[q] = max3(mq[q], __uint_as_float(x[8 * q + 5]), __uint_as_float(x[8 * q + 6]));
-            mq[q] = fmaxf(mq[q], __uint_as_float(x[8 * q + 7]));
+            mq[q] = max3_nan(__uint_as_float(x[8 * q]), __uint_as_float(x[8 * q + 1]), __uint_as_float(x[8 * q + 2]));
+            mq[q] = max3_nan(mq[q], __uint_as_float(x[8 * q + 3]), __uint_as_float(x[8 * q + 4]));
+            mq[q] = max3_nan(mq[q], __uint_as_float(x[8 * q + 5]), __uint_as_float(x[8 * q + 6]));
+            mq[q] = max3_nan(mq[q], mq[q], __uint_as_float(x[8 * q + 7]));
           }
-          mx = max3(mx, max3(mq[0], mq[1], mq[2]), mq[3]);
+          mx = max3_nan(mx, max3_nan(mq[0], mq[1], mq[2]), mq[3]);
         };
 #pragma unroll 1
         for (int c = 0; c < 128; c += 64) {
@@ -706,6 +712,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         }
         if (I8 || masked) tmem_st_wait();
         tmem_ld32_issue(s_addr, x0);
+        // A score that is no number makes the row's sum none either. (It would be lost in the polynomial of the exponentials.)
+        if (mx != mx) l = mx;
         const float m_cand = fmaxf(m, mx);
         const bool grow = (m_cand - m) * c > kChunkLazy;  // -inf -> finite: true; -inf -> -inf is NaN: false
         const float m_new = grow ? m_cand : m;
@@ -843,9 +851,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         if (!ok) continue;
         tc_fence_after();
       }
-      const bool seen = any && m != -INFINITY;  // the row met a key
+      const bool seen = any && !(l == 0.f);  // the row met a key (a score that is no number leaves l no number either)
       if (P.splits > 1) {  // joined below
-        ml_s[row] = seen ? m * c + lv : -INFINITY;
+        ml_s[row] = seen ? (m == -INFINITY ? 0.f : m * c) + lv : -INFINITY;
         ml_s[kChunkRows + row] = l;
         continue;
       }

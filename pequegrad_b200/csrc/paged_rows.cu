@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
         dst[d + kCol * (2 * t + 1)] = o[i][2 * r + 1];
       }
       if (t == 0) {
-        part_m[warp * 16 + row] = m[r] + lv;
+        part_m[warp * 16 + row] = m[r] == -INFINITY && !(l[r] == 0.f) ? 0.f : m[r] + lv;  // a score that is no number: so is l
         part_l[warp * 16 + row] = l[r];
       }
     }

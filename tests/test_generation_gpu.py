@@ -278,6 +278,122 @@ def test_keys_without_a_page_are_left_out(new, ctx, cache):
     check(plan, attend(plan, q, c), q, c)
 
 
+@pytest.mark.parametrize("dtype,cache,D,P", [(F16, F16, 64, 16), (BF16, BF16, 128, 64), (BF16, BF16, 64, 32), (F16, F16, 128, 16), (F16, I8, 64, 32), (BF16, I8, 128, 128)])
+@pytest.mark.parametrize("new,ctx", [(3, 40), (16, 16), (9, 137), (200, 200), (260, 700), (130, 3000)])
+def test_a_token_that_is_not_a_number_reaches_only_the_rows_that_see_it(new, ctx, dtype, cache, D, P):
+    """NaN and infinities in the values (int8: in the scales) and in the keys of new tokens. The rows before such a token give
+    what they would without it; of the rows that see it, a bad value spoils its column, a bad key or scale the row."""
+    H, plan = 2, Plan([new], [ctx], P)
+    k, v = randn(ctx, H, D, dtype=dtype, seed=1), randn(ctx, H, D, dtype=dtype, seed=2)
+    q = randn(new, H, D, dtype=dtype, seed=3)
+    full = Plan([ctx], [ctx], P)
+    first = ctx - new
+    for where in sorted({new - 1, new // 2, 1}):
+        at = first + where
+        for what in ("v nan", "v inf", "v both", "k nan"):
+            c = new_cache(plan, H, D, cache)
+            K.kv_write(k, v, c[0], c[1], full.q_start, full.ctx_len, plan.table, c[2], c[3])
+            want, mass, size = attention_64(plan, q, c, D ** -0.5)
+            bad = v.clone() if what[0] == "v" else k.clone()
+            if what == "v nan":
+                bad[at, 0, 5] = float("nan")
+            elif what == "v inf":
+                bad[at, 1, D - 1], bad[at, 0, 0] = float("-inf"), float("inf")
+            elif what == "v both":
+                bad[at, 0, 7], bad[at - 1, 0, 7] = float("inf"), float("-inf")
+            else:
+                bad[at, 1, 3] = float("nan")
+            K.kv_write(bad if what[0] == "k" else k, bad if what[0] == "v" else v, c[0], c[1], full.q_start, full.ctx_len, plan.table, c[2], c[3])
+            got = attend(plan, q, c)
+            clean = torch.ones((new, H, D), dtype=torch.bool, device="cuda")
+            if cache == I8:  # a head with such a value has no int8 form: all of it reads as NaN
+                heads = {"v nan": [0], "v inf": [0, 1], "v both": [0], "k nan": [1]}[what]
+                clean[max(0, where - (what == "v both")):, heads] = False
+                expect = torch.full_like(want, float("nan"))
+            else:
+                expect = torch.zeros_like(want)
+                if what == "k nan":
+                    expect[where:, 1] = float("nan")
+                    clean[where:, 1] = False
+                else:
+                    for j in (at - 1, at):
+                        b = bad[j].double()
+                        spoilt = ~torch.isfinite(b)
+                        rows = slice(max(0, j - first), None)
+                        expect[rows] += torch.where(spoilt, b, torch.zeros_like(b))
+                        clean[rows] &= ~spoilt
+            bound = attention_bound(want, mass, size, dtype, D, ctx, float(mass.max()) * 4 + 1)
+            err = (got.double() - want).abs()
+            assert bool((err <= bound)[clean].all()), (what, where)
+            g, e = got.double()[~clean], expect[~clean]
+            assert torch.equal(g.isnan(), e.isnan()) and torch.equal(g[~e.isnan()], e[~e.isnan()]), (what, where)
+
+
+@pytest.mark.parametrize("new,ctx", [([1, 2], [100, 40]), ([130], [130]), ([20, 0, 70], [500, 3, 70])])
+@pytest.mark.parametrize("Hq,Hkv,cache,D", [(20, 1, F16, 64), (48, 2, I8, 128), (64, 1, BF16, 128), (17, 1, I8, 64)])
+def test_many_query_heads_share_a_key_head(new, ctx, Hq, Hkv, cache, D):
+    # more than sixteen heads of one token, and numbers that divide no tile
+    dtype = BF16 if cache == BF16 else F16
+    plan = Plan(new, ctx, 32, pad_rows=1)
+    c = new_cache(plan, Hkv, D, cache)
+    q = randn(plan.rows, Hq, D, dtype=dtype)
+    check(plan, attend(plan, q, c), q, c)
+
+
+def test_two_streams_at_once_and_nothing_at_all():
+    plans = [Plan([1] * 30, [300 + 10 * i for i in range(30)], 16, seed=1), Plan([200, 90], [700, 800], 64, seed=2)]
+    work = []
+    for plan, (Hq, Hkv, D, cache) in zip(plans, ((12, 12, 64, F16), (8, 2, 128, I8))):
+        c = new_cache(plan, Hkv, D, cache)
+        q = randn(plan.rows, Hq, D)
+        work.append((plan, q, c, attend(plan, q, c)))
+    streams = [torch.cuda.Stream() for _ in work]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(5):
+        for i, (plan, q, c, _) in enumerate(work):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(attend(plan, q, c))
+    torch.cuda.synchronize()
+    for i, (plan, q, c, alone) in enumerate(work):
+        check(plan, alone, q, c)
+        assert all(same(o, alone) for o in outs[i])
+    # no rows; no sequences; sequences without rows; a cache without pages
+    for new, ctx, pad in (([], [], 0), ([], [], 3), ([0, 0], [5, 0], 2)):
+        plan = Plan(new, ctx, 16, pad_rows=pad)
+        c = new_cache(plan, 2, 64, F16)
+        q = randn(plan.rows, 2, 64)
+        out = torch.full_like(q, 7)
+        attend(plan, q, c, out=out)
+        assert (out == 7).all()
+    plan = Plan([3, 200], [3, 200], 16)
+    c = tuple(torch.empty((0, 2, 16, 64), dtype=F16, device="cuda") for _ in range(2)) + (None, None)
+    assert (attend(plan, randn(203, 2, 64), c) == 0).all()
+    K.kv_write(randn(203, 2, 64), randn(203, 2, 64), c[0], c[1], plan.q_start, plan.ctx_len, plan.table)
+    assert (K.kv_read(c[0], c[1], plan.kv_start, plan.table, 203)[0] == 0).all()
+
+
+@pytest.mark.parametrize("cache", [F16, I8])
+def test_a_wait_that_runs_out_is_reported(cache):
+    """The next chunk launch loads nothing and its waits give up early: it records who gave up and returns, in clusters too;
+    launches do nothing until the word is cleared, and then the same call is right again."""
+    for new, ctx, H in (([200], [2000], 2), ([300] * 6, [300] * 6, 40)):
+        plan = Plan(new, ctx, 32)
+        c = new_cache(plan, H, 64, cache)
+        q = randn(plan.rows, H, 64)
+        check(plan, attend(plan, q, c), q, c)
+        K.gemm_wait_drill(1024, skip_loads=True)
+        out = torch.full_like(q, 7)
+        attend(plan, q, c, out=out)
+        torch.cuda.synchronize()
+        again = torch.full_like(q, 7)
+        attend(plan, q, c, out=again)
+        torch.cuda.synchronize()
+        code = K.device_error(reset=True)
+        assert 32 <= code >> 16 <= 47 and (out == 7).all() and (again == 7).all()
+        check(plan, attend(plan, q, c), q, c)
+
+
 def test_many_sequences_and_heads():
     # more work than the GPU holds at once, of very different lengths
     for new, P, form in ([1] * 200, 16, (F16, F16, 64, 12, 12)), ([1, 90, 2, 0, 33, 1, 128] * 12, 64, (BF16, BF16, 128, 8, 2)), ([5, 1, 20] * 40, 32, (F16, I8, 64, 12, 4)):
