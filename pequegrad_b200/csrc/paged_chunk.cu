@@ -218,11 +218,10 @@ __device__ __forceinline__ void chunk_ld_wait(uint32_t (&v)[32]) {
                  "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]),
                  "+r"(v[31])::"memory");
 }
-// exponent all ones in either half of a word of two 16-bit floats
+// Bit 15 or 31 of the result is set where the low or high 16-bit float of w has an exponent of all ones: NaN or infinity.
 template <bool HALF>
-__device__ __forceinline__ bool not_finite2(uint32_t w) {
-  constexpr uint32_t e = HALF ? 0x7c00u : 0x7f80u;
-  return (w & e) == e || ((w >> 16) & e) == e;
+__device__ __forceinline__ uint32_t exponent_carry(uint32_t w) {
+  return (w & (HALF ? 0x7c007c00u : 0x7f807f80u)) + (HALF ? 0x04000400u : 0x00800080u);
 }
 template <bool HALF>
 __device__ __forceinline__ float half_of(uint32_t w, int hi) {
@@ -308,17 +307,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     const int pr = it.sub + row, tok = chunk_div(pr, P.a.group);
     return P.a.out + ((int64_t)it.token + tok) * P.a.o_row + ((int64_t)it.head * P.a.group + (pr - tok * P.a.group)) * P.a.o_head;
   };
-  // Sixteen columns of a row of O from tensor memory, and, rarely, what was cleared from the values it sees given back.
-  auto load_o = [&](const ChunkItem &it, uint32_t o_addr, int q4, bool any, bool seen, bool slow, int lim, float (&o)[16]) {
+  // 32 columns of a row of O from tensor memory, and, rarely, what was cleared from the values it sees given back.
+  auto load_o = [&](const ChunkItem &it, uint32_t o_addr, int q, bool any, bool seen, bool slow, int lim, float (&o)[32]) {
     if (any) {
-      uint32_t r[16];
-      tmem_ld16_issue(o_addr + q4 * 16, r);
-      tmem_ld_wait();
+      uint32_t r[32];
+      tmem_ld32_issue(o_addr + q * 32, r);
+      chunk_ld_wait(r);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[i] = seen ? __uint_as_float(r[i]) : 0.f;
+      for (int i = 0; i < 32; ++i) o[i] = seen ? __uint_as_float(r[i]) : 0.f;
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[i] = 0.f;
+      for (int i = 0; i < 32; ++i) o[i] = 0.f;
     }
     if (slow) {
       const int end = min(min(lim + 1, it.n_keys), (it.lo + it.steps) << 7);
@@ -326,9 +325,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         const int page = kv_page(P.p, P.c, it.seq, key);
         if (page < 0) continue;
         const int sl = key & ((1 << P.c.log2_page) - 1);
-        const uint32_t *v = reinterpret_cast<const uint32_t *>(P.c.v.base + page * P.c.v.page + it.head * P.c.v.head + sl * P.c.v.slot) + q4 * 8;
+        const uint32_t *v = reinterpret_cast<const uint32_t *>(P.c.v.base + page * P.c.v.page + it.head * P.c.v.head + sl * P.c.v.slot) + q * 16;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < 32; ++i) {
           const float x = half_of<HALF>(v[i >> 1], i & 1);
           if (!(fabsf(x) <= 3.4028234e38f)) o[i] += x;
         }
@@ -430,7 +429,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     const int h = warp - 12;
     const uint32_t idesc_s = attn_idesc(HALF, false, 128), idesc_pv = attn_idesc(HALF, true, D);
     const uint32_t t_s = tmem + h * 128, t_p = S::kAhead ? tmem + 384 + h * 64 : t_s, t_o = tmem + 256 + h * D;
-    const uint32_t q_at = smem_u32(q_s) + h * (S::kQ / 2);
+    // descriptors of the first tile of each operand; the others differ in the address field alone, by constants
+    const uint64_t d_q = make_kmajor_sw128_desc(smem_u32(q_s) + h * (S::kQ / 2)), d_k = make_kmajor_sw128_desc(smem_u32(k_s));
+    const uint64_t d_v = make_mnmajor_sw128_desc(smem_u32(v_s), 16384);
     bool s_more = false, s_first = true;
     auto s_seek = [&]() {  // the next item with blocks for this CTA
       do {
@@ -457,8 +458,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         if (active) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * 16384;
-            tc_mma<kKind>(t_s, make_kmajor_sw128_desc(q_at + off) + 2 * (kk & 3), make_kmajor_sw128_desc(smem_u32(k_s) + ks * S::kKV + off) + 2 * (kk & 3), idesc_s, kk != 0);
+            const uint32_t off = (kk >> 2) * (16384 >> 4) + 2 * (kk & 3);
+            tc_mma<kKind>(t_s, d_q + off, d_k + ks * (S::kKV >> 4) + off, idesc_s, kk != 0);
           }
           tc_commit(&s_full[h]);
           tc_commit(&k_empty[ks]);
@@ -491,7 +492,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
           if (active) {
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)  // 16 keys per MMA: 8 columns of P, 16 rows of V
-              tc_mma_ts(t_o, t_p + kk * 8, make_mnmajor_sw128_desc(smem_u32(v_s) + vs * S::kKV + kk * 2048, 16384), idesc_pv, (j | kk) != 0);
+              tc_mma_ts(t_o, t_p + kk * 8, d_v + vs * (S::kKV >> 4) + kk * (2048 >> 4), idesc_pv, (j | kk) != 0);
             tc_commit(&pv_done[h]);
             tc_commit(&v_empty[vs]);
           } else {
@@ -810,27 +811,31 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
           if (!ok) continue;
           const int key = key0 + tid;
           uint8_t *vrow = v_s + st * S::kKV + tid * 128;
-          if (key > it.first_seen) {
+          auto piece = [&](int u) { return reinterpret_cast<uint4 *>(vrow + (u >> 3) * 16384 + (u & 7) * 16); };  // in any order
+          if (key >= it.n_keys) {
+#pragma unroll
+            for (int u = 0; u < D / 8; ++u) *piece(u) = make_uint4(0, 0, 0, 0);
+          } else if (key > it.first_seen) {
+            uint32_t hit = 0;
 #pragma unroll
             for (int u = 0; u < D / 8; ++u) {
-              uint4 *at = reinterpret_cast<uint4 *>(vrow + (u >> 3) * 16384 + (u & 7) * 16);  // the order in the row does not matter
-              if (key >= it.n_keys) {
-                *at = make_uint4(0, 0, 0, 0);
-              } else {
-                uint4 x = *at;
+              const uint4 x = *piece(u);
+              hit |= exponent_carry<HALF>(x.x) | exponent_carry<HALF>(x.y) | exponent_carry<HALF>(x.z) | exponent_carry<HALF>(x.w);
+            }
+            if (hit & 0x80008000u) {
+              *poison = 1;
+              __threadfence_block();
+#pragma unroll 1
+              for (int u = 0; u < D / 8; ++u) {
+                uint4 x = *piece(u);
                 uint32_t *x4 = reinterpret_cast<uint32_t *>(&x);
-                bool hit = false;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) hit |= not_finite2<HALF>(x4[e]);
-                if (hit) {
-                  *poison = 1;
-                  __threadfence_block();
-                  for (int e = 0; e < 4; ++e) {
-                    if (not_finite2<HALF>(x4[e] & 0xffffu)) x4[e] &= 0xffff0000u;
-                    if (not_finite2<HALF>(x4[e] & 0xffff0000u)) x4[e] &= 0xffffu;
-                  }
-                  *at = x;
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t bad = exponent_carry<HALF>(x4[e]);
+                  if (bad & 0x8000u) x4[e] &= 0xffff0000u;
+                  if (bad & 0x80000000u) x4[e] &= 0xffffu;
                 }
+                *piece(u) = x;
               }
             }
           }
@@ -861,16 +866,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       const bool slow = !I8 && any && *poison != 0;
       uint8_t *out = out_row(it, row);
 #pragma unroll 1
-      for (int q4 = 0; q4 < D / 16; ++q4) {
-        float o[16];
-        load_o(it, o_addr, q4, any, seen, slow, lim, o);
+      for (int q = 0; q < D / 32; ++q) {
+        float o[32];
+        load_o(it, o_addr, q, any, seen, slow, lim, o);
         if (row < it.rows) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < 4; ++i) {
             uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) w[k] = out_pair<HALF>(o[8 * i + 2 * k] * inv, o[8 * i + 2 * k + 1] * inv);
-            *reinterpret_cast<uint4 *>(out + q4 * 32 + i * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4 *>(out + q * 64 + i * 16) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
       }
@@ -902,13 +907,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     const uint32_t o_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 256 + h * D;
     const int lim = last_seen(it, row);
     const bool slow = !I8 && any && *poison != 0;
-#pragma unroll 2
-    for (int q4 = 0; q4 < D / 16; ++q4) {
-      float o[16];
-      load_o(it, o_addr, q4, any, seen, slow, lim, o);
-      float4 *st = reinterpret_cast<float4 *>(k_s) + q4 * 4 * kChunkRows + row;
+#pragma unroll 1
+    for (int q = 0; q < D / 32; ++q) {
+      float o[32];
+      load_o(it, o_addr, q, any, seen, slow, lim, o);
+      float4 *st = reinterpret_cast<float4 *>(k_s) + q * 8 * kChunkRows + row;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) st[i * kChunkRows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+      for (int i = 0; i < 8; ++i) st[i * kChunkRows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
     }
   }
   tc_fence_before();
