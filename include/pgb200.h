@@ -325,7 +325,8 @@ PGB_API int pgb_quantize_i8(const pgb_tensor *x, const float *absmax_dev, float 
 /* Error word of the kernels' bounded device-side waits (every mbarrier wait of the tensor-core GEMMs and of the fused
  * attention gives up after a fixed number of polls instead of hanging). Synchronises with the device. *code = 0 and
  * PGB_OK when no wait ran out; else *code = (role << 16) | block (roles: 1 producer, 2 MMA issuer, 3 epilogue of the
- * GEMM kernels; 10, 11 the peer collectives; 16-26 the attention kernel's producer, MMA issuer and softmax waits) and
+ * GEMM kernels; 10, 11 the peer collectives; 16-26 the attention kernel's producer, MMA issuer and softmax waits; 32-47
+ * those of the attention over the paged cache) and
  * the return value is PGB_ERR_TIMEOUT. While the word is set, later launches of those kernels return at once without
  * computing; `reset` clears it. Replaces nothing in the reference, whose kernels never wait on one another. */
 PGB_API int pgb_device_error(int *code, int reset);
@@ -337,7 +338,7 @@ PGB_API int pgb_device_error(int *code, int reset);
  * Returns the previous mode. A tuning switch in the manner of cublasSetMathMode; the reference has no counterpart. */
 PGB_API int pgb_gemm_pair_mode(int mode);
 
-/* Failure-detection drill: the NEXT tensor-core GEMM or fused attention launched from this host thread polls each of
+/* Failure-detection drill: the NEXT tensor-core GEMM, fused attention or chunk kernel of the paged attention launched from this host thread polls each of
  * its waits at most `polls` times and, with skip_loads != 0, its producer issues no loads, so the wait of its MMA
  * warp runs out: the kernel records the error word above, frees its tensor memory and returns; nothing faults or
  * hangs. Used by the tests to exercise the timeout path; no counterpart in the reference. */

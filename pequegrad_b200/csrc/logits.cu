@@ -9,6 +9,10 @@
 // The work is one read and one write of the logits; the counts never leave the SM: a CTA owns a slice of one row's
 // vocabulary, counts the history's tokens that fall into it with integer atomics in shared memory (their order does not
 // change the result), and then streams its slice. Every CTA of a row reads the whole history, which the L2 serves.
+//
+// 256 rows of 50257 halves with histories of up to 2000 tokens, 64 biases and a mask: 35 us (54 MB: 8 us at the copy rate). The
+// copy alone takes 16 us through shared memory (results at another alignment than the logits), the history 10: thirteen CTAs
+// of a row read it, and a CTA's chain of loads, atomics and two barriers is a few microseconds, of which 4 to 6 overlap on an SM.
 #include <cstring>
 #include <string>
 
