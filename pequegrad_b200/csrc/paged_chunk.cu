@@ -95,7 +95,7 @@ struct ChunkItem {
 __device__ __forceinline__ int chunk_div(int x, int group) { return group == 1 ? x : (int)((unsigned)x / (unsigned)group); }
 
 struct ChunkCursor {
-  int hi = 0, lo = 0;  // tiles with keys in (lo, hi] are being dealt out; hi == 0: not begun
+  int hi = -1, lo = 0;  // tiles with keys in (lo, hi] are being dealt out; hi < 0: not begun
   int seq0 = 0, base = 0;
 };
 
@@ -108,7 +108,7 @@ __device__ __forceinline__ bool chunk_item(const ChunkParams &P, int id, int ran
   const int lane = threadIdx.x & 31;
   const int t = id / P.c.heads;
   it.head = id - t * P.c.heads;
-  if (cur.hi == 0) {
+  if (cur.hi < 0) {
     int most = 0;
     for (int s = lane; s < P.p.n_seq; s += 32) most = max(most, __ldg(P.p.ctx + s));
     most = __reduce_max_sync(0xffffffffu, most);
@@ -341,9 +341,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       }
     }
   };
+  // Some wait for a whole item, which a context of 2^30 tokens makes seconds long. Each ends when a role that waits for one
+  // step at a time ends, or gives up and raises the flag that every wait looks at.
+  const uint32_t patient = P.polls < (1u << 20) ? P.polls : 1u << 31;
   // a wait of the whole warp; `role` goes into the error word
-  auto wait = [&](uint64_t *bar, uint32_t parity, int role) -> bool {
-    const bool ok = __all_sync(0xffffffffu, attn_wait(bar, parity, abort_flag, P.polls));
+  auto wait = [&](uint64_t *bar, uint32_t parity, int role, uint32_t polls = 0) -> bool {
+    const bool ok = __all_sync(0xffffffffu, attn_wait(bar, parity, abort_flag, polls ? polls : P.polls));
     if (!ok && lane == 0) {
       *abort_flag = 1;
       atomicCAS(P.err, 0, (role << 16) | (int)(blockIdx.x & 0xffff));
@@ -363,7 +366,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
   // The next item; false past the last. In a cluster a role does one item between two joins.
   auto read_item = [&](uint32_t &count, ChunkItem &to, bool release) -> bool {
     const uint32_t slot = count % kItemSlots;
-    if (!wait(&item_full[slot], (count / kItemSlots) & 1, 46)) { ok = false; return false; }
+    if (!wait(&item_full[slot], (count / kItemSlots) & 1, 46, patient)) { ok = false; return false; }
     const int4 a = item_s[4 * slot], b = item_s[4 * slot + 1], c = item_s[4 * slot + 2];
     if (release) {
       __syncwarp();
@@ -387,7 +390,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     const int u = (w * 32 + lane) % kUnits, step_tok = chunk_div(kRows, P.a.group), step_head = kRows - step_tok * P.a.group;
     while (take()) {
       if (it.steps == 0) continue;
-      if (!(ok = wait(q_empty, (n & 1) ^ 1, 32))) break;
+      if (!(ok = wait(q_empty, (n & 1) ^ 1, 32, patient))) break;
       ++n;
       int row = (w * 32 + lane) / kUnits;
       int tok = chunk_div(it.sub + row, P.a.group), head = it.sub + row - tok * P.a.group;
@@ -414,7 +417,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         const int id = id_of((int)taken);
         more = id < n_items && chunk_item(P, id, rank, cur, it);
         const uint32_t slot = taken % kItemSlots;
-        if (!(ok = wait(&item_empty[slot], ((taken / kItemSlots) & 1) ^ 1, 47))) break;
+        if (!(ok = wait(&item_empty[slot], ((taken / kItemSlots) & 1) ^ 1, 47, patient))) break;
         if (lane == 0) {
           item_s[4 * slot] = make_int4(more ? it.seq : -1, it.head, it.token, it.sub);
           item_s[4 * slot + 1] = make_int4(it.rows, it.pos, it.n_keys, it.first_seen);

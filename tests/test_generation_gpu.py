@@ -152,7 +152,7 @@ def check(plan, got, q, cache, scale=None):
     want, mass, size = attention_64(plan, q, cache, D ** -0.5 if scale is None else scale)
     n = plan.starts[-1]
     vmax = float(mass.max()) * 4 + 1 if mass.numel() else 1.0
-    bound = attention_bound(want, mass, size, q.dtype, D, max(plan.ctx, default=0), vmax)
+    bound = attention_bound(want, mass, size, q.dtype, D, max(0, max(plan.ctx, default=0)), vmax)
     err = (got.double() - want).abs()
     bad = ~(err <= bound)[:n]
     assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, worst {float((err - bound)[:n].max()):.3g} at {bad.nonzero()[0].tolist()}"
@@ -428,6 +428,46 @@ def test_a_long_context_and_pages_past_four_gigabytes():
         p.table_list, p.pages, p.table = plan.table_list, pages, plan.table
         q = randn(new, H, D)
         check(p, attend(p, q, (kc, vc, None, None)), q, (kc, vc, None, None))
+
+
+def test_contexts_shorter_than_their_new_rows():
+    # more sequences than a warp looks at together, none of which has a key for any row; then some that have
+    for ctx in ([0] * 45, [-3] * 40, [0] * 33 + [25] * 20):
+        for new in (1, 20, 300):
+            plan = Plan([new] * len(ctx), ctx, 16, pad_rows=1)
+            c = new_cache(plan, 2, 64, F16)
+            q = randn(plan.rows, 2, 64)
+            out = torch.full_like(q, 7)
+            attend(plan, q, c, out=out)
+            check(plan, out, q, c)
+            assert (out[: new * ctx.count(ctx[0])] == 0).all() and (out[-1] == 7).all()
+
+
+@pytest.mark.parametrize("cache", [F16, I8])
+@pytest.mark.parametrize("new", [1, 32])
+def test_a_context_of_millions_of_tokens(new, cache):
+    """A table that names one page over and over: key j of the page counts as often as it is seen. A role may wait for as long
+    as an item takes, which here is tens of milliseconds, and the second item of a CTA as long again."""
+    D, P, H = 64, 128, 160
+    ctx = (1 << 22) + 37
+    plan = Plan([new], [ctx], P, spare_pages=0)
+    plan.pages = 1
+    plan.table = torch.zeros_like(plan.table)
+    c = new_cache(plan, H, D, cache)
+    q = randn(new, H, D, seed=9)
+    out = attend(plan, q, c)
+    k, v = (x[0].double() * (1.0 if s is None else s[0].double()[..., None]) for x, s in ((c[0], c[2]), (c[1], c[3])))
+    pos = torch.arange(ctx - new, ctx, device="cuda")
+    times = (pos // P)[:, None] + (torch.arange(P, device="cuda") <= (pos % P)[:, None])
+    score = torch.einsum("nhd,hjd->nhj", q.double(), k) * D ** -0.5
+    p = torch.softmax(score + torch.log(times.double())[:, None], -1)
+    want, mass = torch.einsum("nhj,hjd->nhd", p, v), torch.einsum("nhj,hjd->nhd", p, v.abs())
+    size = float((torch.einsum("nhd,hjd->nhj", q.double().abs(), k.abs()) * D ** -0.5).max())
+    # beside the usual bound: fp32 sums of millions of terms, added in an order of at most 2^17 partial sums a row
+    bound = attention_bound(want, mass, size, F16, D, 0, 0.0) + 2.0 ** 17 * 2.0 ** -24 * mass
+    err = (out.double() - want).abs()
+    assert bool((err <= bound).all()), float((err - bound).max())
+    assert K.device_error() == 0
 
 
 # ---- logits ----------------------------------------------------------------------------------------------------------
