@@ -151,7 +151,7 @@ def make_tensor(ptr: int, dtype: int, shape, stride_bytes) -> PgbTensor:
 
 
 # PgbTensor's layout by number of dims: data, dtype, ndim, shape[MAX_DIMS], stride_bytes[MAX_DIMS]
-_PACKED = [struct.Struct(f"<Qii{n}q{8 * (MAX_DIMS - n)}x{n}q{8 * (MAX_DIMS - n)}x") for n in range(MAX_DIMS + 1)]
+PACKED = [struct.Struct(f"<Qii{n}q{8 * (MAX_DIMS - n)}x{n}q{8 * (MAX_DIMS - n)}x").pack for n in range(MAX_DIMS + 1)]
 
 
 def pack_tensor(ptr: int, dtype: int, shape, stride_bytes) -> bytes:
@@ -159,7 +159,7 @@ def pack_tensor(ptr: int, dtype: int, shape, stride_bytes) -> bytes:
     n = len(shape)
     if n > MAX_DIMS:
         raise ValueError("at most 8 dims are supported")
-    return _PACKED[n].pack(ptr, dtype, n, *shape, *stride_bytes)
+    return PACKED[n](ptr, dtype, n, *shape, *stride_bytes)
 
 
 def make_program(instrs) -> tuple:

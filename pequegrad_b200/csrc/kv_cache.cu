@@ -151,6 +151,21 @@ __device__ __forceinline__ void row_and_head(int64_t g, int64_t rows, int heads,
   }
 }
 
+// For the read: TILE consecutive rows of one head, then the next head, so that a warp reads one stretch of a page. The rows that
+// fill no tile come last, head by head.
+template <int TILE>
+__device__ __forceinline__ void row_and_head_tiled(int64_t g, int64_t rows, int heads, int64_t &row, int &head) {
+  const int64_t whole = rows - rows % TILE;
+  if (g >= whole * heads) {
+    row_and_head(g - whole * heads, rows - whole, heads, row, head);
+    row += whole;
+    return;
+  }
+  int64_t block;
+  row_and_head(g / TILE, whole / TILE, heads, block, head);
+  row = block * TILE + g % TILE;
+}
+
 // Eight 16-bit values as fp32, and back.
 template <bool HALF>
 __device__ __forceinline__ void widen8(const uint4 &r, float (&x)[8]) {
@@ -264,8 +279,8 @@ __device__ __forceinline__ void store_dequantised(uint8_t *dst, const uint4 &r, 
 }
 
 // The mirror image of the store: a lane moves 16 bytes of K and of V (eight 16-bit or sixteen int8 values). 12 sequences of up
-// to 8192 int8 tokens, 8 heads of 128, into bf16: 73 us, 0.71 of the copy rate; two and four rows a thread, with all their
-// loads under way at once, took 74 and 82.
+// to 8192 int8 tokens, 8 heads of 128, into bf16: 68 us, 0.77 of the copy rate (73 with a warp across four heads of a token). Two
+// and four rows a thread, with all their loads under way at once, were slower (74 and 82 against 73).
 template <int D, bool I8, int OUT>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvRows y, const __grid_constant__ KvCache c,
                                                       const __grid_constant__ KvPlan p) {
@@ -276,7 +291,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Kv
   if (g >= y.rows * c.heads) return;
   int64_t row;
   int head;
-  row_and_head(g, y.rows, c.heads, row, head);
+  row_and_head_tiled<32 / kLanes>(g, y.rows, c.heads, row, head);
   const int s = kv_sequence(p, row);
   if (s < 0) return;  // behind the last sequence: left as it was
   const int64_t pos = kv_position(p, s, row);

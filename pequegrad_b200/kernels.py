@@ -274,21 +274,27 @@ _DTYPE_SIZE = {dt: (code, torch.empty((), dtype=dt).element_size()) for dt, code
 
 
 def _packed(ref: torch.Tensor, tensors) -> list:
-    """Descriptors of tensors (None stays None) that must lie on `ref`'s device."""
+    """Descriptors of tensors (None stays None) that must lie on `ref`'s device: `_lib.pack_tensor` of each, written out
+    because small calls take less time on the GPU than here."""
     dev = ref.get_device()
-    if not ref.is_cuda:
+    if dev < 0:
         raise RuntimeError("pgb200 kernels need CUDA tensors: there is no CPU path")
-    out = []
+    out, packed = [], L.PACKED
     for t in tensors:
         if t is None:
             out.append(None)
             continue
         if t.get_device() != dev:
             raise ValueError(f"all tensors must be on one device: {t.device} and {ref.device}")
-        if t.dtype not in _DTYPE_SIZE:
+        try:
+            code, size = _DTYPE_SIZE[t.dtype]
+        except KeyError:
             pgb_dtype(t.dtype)  # raises
-        code, size = _DTYPE_SIZE[t.dtype]
-        out.append(L.pack_tensor(t.data_ptr(), code, t.shape, [s * size for s in t.stride()]))
+        shape = t.shape
+        n = len(shape)
+        if n > L.MAX_DIMS:
+            raise ValueError("at most 8 dims are supported")
+        out.append(packed[n](t.data_ptr(), code, n, *shape, *[s * size for s in t.stride()]))
     return out
 
 
