@@ -12,7 +12,8 @@
 //                   int8: each warp brings 32 keys a block into a raw ring with cp.async, widens them exactly to 16 bits and
 //                   stores them as the tiles TMA would have written; scales go to the softmax warps through a small ring.
 //   warps 12, 13    issue the MMAs of A and of B (one lane each), so that neither half waits for the other's softmax
-//   warp 14         Q rows, by cp.async into the swizzled tiles (warps 9-11 help where keys come by TMA)
+//   warp 14         Q: where the group divides 128, by TMA (a box of group heads x 128 / group tokens is a half); otherwise by
+//                   cp.async into the swizzled tiles (warps 9-11 help where keys come by TMA)
 //   warp 15         finds the items, some ahead of their use: the search's loads and divisions stay out of the other roles' way
 //                   and its code is there once
 // Tensor memory: S_A [0, 128), S_B [128, 256), O_A, O_B behind them. With head dim 64 there is room for P beside S, and the
@@ -28,7 +29,7 @@
 // Bound by the latency of a softmax warp's chain (two warps a scheduler) more than by either pipe. A step of 256 rows and 128
 // keys takes 2.0 us with head dim 64 (610 TFLOP/s over the GPU, the tensor pipe at a fifth of its cycles in a profile),
 // 3.2 us with 128 (780 TFLOP/s; S waits for the product that reads P), 3.3 and 5 us beside an int8 cache, whose scales are
-// read and multiplied twice a score. A launch and its first item cost 11 us before and behind the steps, each further item 4.
+// read and multiplied twice a score. A launch and its first item cost 10 us before and behind the steps, each further item 4.
 // Tried and slower: 128 scores held in registers (spills, 4.7 us a step with head dim 64, and the code leaves the instruction
 // cache); one MMA warp for both halves; every role searching its items itself (74 against 50 us for 8 x 1024 tokens).
 #include <cuda_bf16.h>
@@ -76,6 +77,7 @@ struct ChunkParams {
   int *err;
   uint32_t polls;
   int skip_loads;
+  int q_tma;  // Q has a tensor map
 };
 
 struct ChunkItem {
@@ -170,14 +172,6 @@ __device__ __forceinline__ bool chunk_item(const ChunkParams &P, int id, int ran
     it.steps = n_all * (rank + 1) / P.splits - it.lo;
     it.n_a = max(0, min(it.steps, n_a - it.lo));
     it.n_b = it.rows > 128 ? it.steps : 0;
-    // every lane has the same values; a broadcast tells the compiler so
-    it.steps = __shfl_sync(0xffffffffu, it.steps, 0);
-    it.n_a = __shfl_sync(0xffffffffu, it.n_a, 0);
-    it.n_b = __shfl_sync(0xffffffffu, it.n_b, 0);
-    it.lo = __shfl_sync(0xffffffffu, it.lo, 0);
-    it.seq = __shfl_sync(0xffffffffu, it.seq, 0);
-    it.first_seen = __shfl_sync(0xffffffffu, it.first_seen, 0);
-    it.n_keys = __shfl_sync(0xffffffffu, it.n_keys, 0);
     return true;
   }
 }
@@ -238,7 +232,7 @@ __device__ __forceinline__ float half_of(uint32_t w, int hi) {
 }
 
 template <bool HALF, int D, bool I8>
-__global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+__global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                        const __grid_constant__ ChunkParams P) {
   using S = ChunkTile<D, I8>;
   constexpr int kQWarps = I8 ? 1 : 4;  // 14 and, where keys come by TMA, 9-11
@@ -257,8 +251,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
   uint64_t *k_full = bars + 2, *k_empty = k_full + 4, *v_full = k_empty + 4, *v_empty = v_full + 4;  // [kStages]
   uint64_t *sc_full = v_empty + 4, *sc_empty = sc_full + kScaleSlots;
   uint64_t *s_full = sc_empty + kScaleSlots, *s_free = s_full + 2, *p_full = s_free + 2, *pv_done = p_full + 2;  // [half]
-  uint64_t *item_full = pv_done + 2, *item_empty = item_full + kItemSlots;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(item_empty + kItemSlots);
+  uint64_t *item_full = pv_done + 2, *item_empty = item_full + kItemSlots, *drained = item_empty + kItemSlots;  // drained: [half]
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 2);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   int *dead = const_cast<int *>(abort_flag) + 1;
   volatile int *poison = const_cast<volatile int *>(abort_flag) + 2;
@@ -272,7 +266,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
   auto id_of = [&](int r) -> int { return r * units + ((r & 1) ? units - 1 - unit : unit); };
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, kQWarps);
+    mbar_init(q_full, P.q_tma ? 1 : kQWarps);
     mbar_init(q_empty, 2);
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(&k_full[s], I8 ? 4 : 1);
@@ -293,6 +287,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       mbar_init(&s_free[h], 4);
       mbar_init(&p_full[h], 4);
       mbar_init(&pv_done[h], 1);
+      mbar_init(&drained[h], 1);
     }
     *abort_flag = 0;
     *poison = 0;
@@ -359,6 +354,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
   uint32_t taken = 0, s_taken = 0;
   uint32_t g = 0, n = 0, s_g = 0, s_n = 0, s_items = 0;
   int s_j = 0;
+  bool gone = false;  // after a wait that ran out, what was in flight has been seen out
   bool ok = run && !(P.skip_loads && (warp == 14 || (warp >= 8 && warp < 12)));
 
   // Alone, a CTA walks all its rounds with every role at its own pace. In a cluster the CTAs meet after each round and join.
@@ -389,9 +385,21 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     constexpr int kUnits = D / 8, kRows = kQWarps * 32 / kUnits;  // pieces of a row; rows at once
     const int u = (w * 32 + lane) % kUnits, step_tok = chunk_div(kRows, P.a.group), step_head = kRows - step_tok * P.a.group;
     while (take()) {
-      if (it.steps == 0) continue;
+      if (it.steps == 0 || (P.q_tma && w > 0)) continue;
       if (!(ok = wait(q_empty, (n & 1) ^ 1, 32, patient))) break;
       ++n;
+      if (P.q_tma) {  // rows of other sequences behind the item's are loaded with it and not used; behind the last row, zeros
+        if (lane == 0) {
+          mbar_expect_tx(q_full, S::kQ);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int d = 0; d < D / 64; ++d)
+              tma_load_4d(q_s + h * (S::kQ / 2) + d * 16384, &map_q, 64 * d, it.head * P.a.group, it.token + h * chunk_div(128, P.a.group), 0, q_full);
+        }
+        __syncwarp();
+        continue;
+      }
       int row = (w * 32 + lane) / kUnits;
       int tok = chunk_div(it.sub + row, P.a.group), head = it.sub + row - tok * P.a.group;
       for (; row < kChunkRows; row += kRows) {
@@ -543,6 +551,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
                 for (int d = 0; d < D / 64; ++d) tma_load_4d(dst + d * 16384, kv ? &map_v : &map_k, 64 * d, 0, it.head, page, full);
               }
               __syncwarp();
+              if (kv) n = g + 1;
+              else s_n = g + 1;  // blocks of V and of K that were asked for
             }
             page = next;
           }
@@ -895,6 +905,27 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
 
   tc_fence_before();
   __syncthreads();
+  if (run && *abort_flag != 0 && !gone) {
+    // Some role gave up. Copies and products that are in flight are waited for, with a limit again: nothing may write the
+    // memory of a CTA that has gone.
+    gone = true;
+    auto see_out = [&](uint64_t *bar, uint32_t parity) {
+      for (uint32_t i = 0; i < kChunkPolls && !mbar_try_wait(bar, parity); ++i) {}
+    };
+    if (!I8 && warp == 8) {
+      for (uint32_t st = 0; st < S::kStages; ++st) {
+        if (s_n > st) see_out(&k_full[(s_n - 1 - st) % S::kStages], ((s_n - 1 - st) / S::kStages) & 1);
+        if (n > st) see_out(&v_full[(n - 1 - st) % S::kStages], ((n - 1 - st) / S::kStages) & 1);
+      }
+    } else if (warp == 14 && P.q_tma) {
+      if (n > 0) see_out(q_full, (n - 1) & 1);
+    } else if (warp == 12 || warp == 13) {
+      if (lane == 0) tc_commit(&drained[warp - 12]);
+      __syncwarp();
+      see_out(&drained[warp - 12], 0);
+    }
+    __syncthreads();
+  }
   if (P.splits == 1) break;
   // The round's item once more, for the warps whose role did not read it. A CTA whose wait ran out writes nothing, but stays
   // for every barrier of its cluster, since the others read its shared memory.
@@ -985,7 +1016,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
 }
 
 template <bool HALF, int D, bool I8>
-static int launch(ChunkParams &P, const CUtensorMap &mk, const CUtensorMap &mv, int64_t items, int64_t blocks, cudaStream_t stream) {
+static int launch(ChunkParams &P, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, int64_t items, int64_t blocks, cudaStream_t stream) {
   using S = ChunkTile<D, I8>;
   const auto kernel = paged_chunk_kernel<HALF, D, I8>;
   int dev = 0;
@@ -1045,7 +1076,7 @@ static int launch(ChunkParams &P, const CUtensorMap &mk, const CUtensorMap &mv, 
   }
   cfg.gridDim = dim3((unsigned)(std::min(items, units) * P.splits));
   attr[0].val.clusterDim.x = P.splits;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mk, mv, P);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, P);
   if (e != cudaSuccess) {
     cudaGetLastError();
     set_error(std::string("paged_chunk_kernel: ") + cudaGetErrorString(e));
@@ -1070,6 +1101,21 @@ static bool page_map(CUtensorMap *m, const KvCache &c, const KvPages &p) {
   return encode_map_4d(m, c.dtype == PGB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.base, dims, strides, box);
 }
 
+// Q as [rows, heads, head dim] with a box of one half's rows: the heads of a group times 128 / group tokens. False where the
+// group does not divide 128 or TMA cannot address Q: its rows are copied one by one then.
+static bool query_map(CUtensorMap *m, const PagedParams &a, const KvCache &c, bool half) {
+  if (128 % a.group) return false;
+  const uint64_t dims[4] = {(uint64_t)c.head_dim, (uint64_t)a.heads, (uint64_t)a.rows, 1};
+  // a dim of extent 1 still needs a valid stride
+  const uint64_t head = a.heads > 1 ? (uint64_t)a.q_head : (uint64_t)c.head_dim * 2;
+  const uint64_t row = a.rows > 1 ? (uint64_t)a.q_row : head * a.heads;
+  const uint64_t strides[3] = {head, row, row};
+  const uint32_t box[4] = {64, (uint32_t)a.group, (uint32_t)(128 / a.group), 1};
+  for (uint64_t s : strides)
+    if (s == 0 || s >= (1ull << 40)) return false;
+  return encode_map_4d(m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.q, dims, strides, box);
+}
+
 bool run_paged_chunk(const PagedParams &a, const KvCache &c, const KvPlan &p, bool half, cudaStream_t stream, int *status) {
   ChunkParams P{};
   P.a = a;
@@ -1078,8 +1124,9 @@ bool run_paged_chunk(const PagedParams &a, const KvCache &c, const KvPlan &p, bo
   // tiles of 256 rows: each sequence that has rows adds at most one that is not full
   const int64_t k = std::min<int64_t>(p.n_seq, a.rows), tiles = (a.rows * a.group - k) / kChunkRows + k;
   if (tiles * c.heads > 1073741824LL || c.n_pages == 0) return false;
-  CUtensorMap mk{}, mv{};
+  CUtensorMap mq{}, mk{}, mv{};
   if (c.dtype != PGB_I8 && (!page_map(&mk, c, c.k) || !page_map(&mv, c, c.v))) return false;
+  P.q_tma = query_map(&mq, a, c, half) ? 1 : 0;
   P.n_tiles = (int)tiles;
   const int64_t items = tiles * c.heads, blocks = ((int64_t)p.width << c.log2_page) / 128;
   P.err = gemm_error_word();
@@ -1092,7 +1139,7 @@ bool run_paged_chunk(const PagedParams &a, const KvCache &c, const KvPlan &p, bo
   take_next_wait_test(&drill_polls, &P.skip_loads);
   P.polls = drill_polls ? drill_polls : kChunkPolls;
   const bool i8 = c.dtype == PGB_I8;
-#define PGB_CHUNK(H, D, Q) launch<H, D, Q>(P, mk, mv, items, blocks, stream)
+#define PGB_CHUNK(H, D, Q) launch<H, D, Q>(P, mq, mk, mv, items, blocks, stream)
   if (half) {
     if (c.head_dim == 64) *status = i8 ? PGB_CHUNK(true, 64, true) : PGB_CHUNK(true, 64, false);
     else *status = i8 ? PGB_CHUNK(true, 128, true) : PGB_CHUNK(true, 128, false);
