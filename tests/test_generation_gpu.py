@@ -607,6 +607,49 @@ def test_a_captured_step_follows_the_plan_in_memory_and_side_streams_work():
             assert same(c[0][page, :, slot], x[b, 1]) and same(c[1][page, :, slot], x[b, 2])
 
 
+FIRST_CALLS = """
+import sys, torch
+sys.path[:0] = sys.argv[1:]
+from generation import Plan, new_cache
+from pequegrad_b200 import kernels as K
+work = []
+for new, cache in (([1, 1], torch.float16), ([40, 90], torch.int8), ([300], torch.float16)):
+    plan = Plan(new, [n + 50 for n in new], 16)
+    c, x = new_cache(plan, 2, 64, cache), torch.randn((plan.rows, 3, 2, 64), device="cuda").half()
+    work.append((plan, c, x, torch.empty((plan.rows, 2, 64), dtype=torch.float16, device="cuda")))
+logits = torch.randn((2, 77), device="cuda")
+shaped = torch.empty_like(logits)
+read = [torch.empty((work[0][0].kv_starts[-1], 2, 64), dtype=torch.float16, device="cuda") for _ in range(2)]
+def step():
+    for p, c, x, o in work:
+        K.kv_write(x[:, 1], x[:, 2], c[0], c[1], p.q_start, p.ctx_len, p.table, c[2], c[3])
+        K.paged_attention(x[:, 0], c[0], c[1], p.q_start, p.ctx_len, p.table, None, c[2], c[3], out=o)
+    p, c = work[0][:2]
+    K.kv_read(c[0], c[1], p.kv_start, p.table, read[0].shape[0], out=read)
+    K.logits_process(logits, bias_ids=p.table[:, :1].contiguous(), bias=torch.ones((2, 1), device="cuda"), out=shaped)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    step()
+graph.replay()
+torch.cuda.synchronize()
+replayed = [t.clone() for t in [w[3] for w in work] + read + [shaped]]
+step()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(replayed, [w[3] for w in work] + read + [shaped])) and K.device_error() == 0
+print("same")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = Path(__file__).resolve().parents[1]
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS, str(root), str(root / "tests")], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.strip() == "same", r.stderr[-2000:]
+
+
 def test_operands_on_two_devices_are_refused():
     plan = Plan([1], [5], 16)
     c = new_cache(plan, 1, 64, F16)
