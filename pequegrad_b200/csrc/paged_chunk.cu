@@ -706,10 +706,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
             }
           }
           if (masked) {
-            const uint32_t gone = absent >> (c >> 4);
+            // a bit for each of the 32 columns: up to the row's last, without the sixteens that have no page
+            const int more = last - c;
+            uint32_t keep = more >= 31 ? 0xffffffffu : more < 0 ? 0u : (2u << more) - 1;
+            if ((absent >> (c >> 4)) & 1) keep &= 0xffff0000u;
+            if ((absent >> (c >> 4)) & 2) keep &= 0xffffu;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (c + i > last || ((gone >> (i >> 4)) & 1)) x[i] = 0xff800000u;  // -inf
+              if (!((keep >> i) & 1)) x[i] = 0xff800000u;  // -inf
           }
           if (I8 || masked) tmem_st32(s_addr + c, x);
           float mq[4];
