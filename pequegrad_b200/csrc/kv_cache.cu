@@ -279,7 +279,7 @@ __device__ __forceinline__ void store_dequantised(uint8_t *dst, const uint4 &r, 
 }
 
 // The mirror image of the store: a lane moves 16 bytes of K and of V (eight 16-bit or sixteen int8 values). 12 sequences of up
-// to 8192 int8 tokens, 8 heads of 128, into bf16: 68 us, 0.77 of the copy rate (73 with a warp across four heads of a token). Two
+// to 8192 int8 tokens, 8 heads of 128, into bf16: 68 to 70 us, 0.75 of the copy rate (73 with a warp across four heads of a token). Two
 // and four rows a thread, with all their loads under way at once, were slower (74 and 82 against 73).
 template <int D, bool I8, int OUT>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvRows y, const __grid_constant__ KvCache c,

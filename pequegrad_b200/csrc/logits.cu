@@ -10,7 +10,7 @@
 // vocabulary, counts the history's tokens that fall into it with integer atomics in shared memory (their order does not
 // change the result), and then streams its slice. Every CTA of a row reads the whole history, which the L2 serves.
 //
-// 256 rows of 50257 halves with histories of up to 2000 tokens, 64 biases and a mask: 35 us (54 MB: 8 us at the copy rate). The
+// 256 rows of 50257 halves with histories of up to 2000 tokens, 64 biases and a mask: 33 us (54 MB: 8 us at the copy rate). The
 // copy alone takes 16 us through shared memory (results at another alignment than the logits), the history 10: thirteen CTAs
 // of a row read it, and a CTA's chain of loads, atomics and two barriers is a few microseconds, of which 4 to 6 overlap on an SM.
 #include <cstring>
@@ -26,7 +26,7 @@ constexpr int kLogitThreads = 256;
 template <typename IoT> constexpr int kLogitSlice = 2 * kLogitThreads * 16 / (int)sizeof(IoT);
 // A shared-memory array of them, with room to shift them as a row's start requires.
 template <typename IoT> constexpr int kLogitRoom = kLogitSlice<IoT> + 8;
-constexpr uint32_t kSeen = 0x80000000u;  // bit 31 of a counter: the token occurs at all; the rest counts the generated ones
+constexpr uint32_t kSeen = 0x80000000u;  // bit 31 of a counter: the token occurs in the prompt; the rest counts the generated ones
 
 struct LogitParams {
   const void *x;
@@ -98,11 +98,8 @@ __global__ void __launch_bounds__(kLogitThreads) logits_kernel(const __grid_cons
     auto put = [&](int i, int id) {
       const int64_t at = (int64_t)id - v0;
       if (at < 0 || at >= n) return;
-      if (i >= prompt) {
-        if ((atomicAdd(count + at, 1u) & kSeen) == 0) atomicOr(count + at, kSeen);
-      } else {
-        atomicOr(count + at, kSeen);
-      }
+      if (i >= prompt) atomicAdd(count + at, 1u);  // a count that is not zero says as much as the flag
+      else atomicOr(count + at, kSeen);
     };
 #pragma unroll
     for (int u = 0; u < 4; ++u)
