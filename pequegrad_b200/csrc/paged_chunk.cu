@@ -451,15 +451,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     // descriptors of the first tile of each operand; the others differ in the address field alone, by constants
     const uint64_t d_q = make_kmajor_sw128_desc(smem_u32(q_s) + h * (S::kQ / 2)), d_k = make_kmajor_sw128_desc(smem_u32(k_s));
     const uint64_t d_v = make_mnmajor_sw128_desc(smem_u32(v_s), 16384);
+    // The cursor of the scores reads items without giving up their slots, which `take` does. So it never looks past the item
+    // behind the last one taken: an item without blocks stops it until `take` has passed that. (Looking for the next item with
+    // blocks through any number of others, it would wait for a slot that this warp holds.) And it reads every item before
+    // `take` does, while the slot is the item's.
     bool s_more = false, s_first = true;
-    auto s_seek = [&]() {  // the next item with blocks for this CTA
-      do {
-        s_more = ok && (P.splits == 1 || s_first) && read_item(s_taken, s_it, false);
+    auto s_seek = [&]() -> bool {
+      while (ok && !s_more && s_taken <= taken && (P.splits == 1 || s_first)) {
         s_first = false;
-      } while (s_more && s_it.steps == 0);
+        s_more = read_item(s_taken, s_it, false) && s_it.steps > 0;
+      }
+      return s_more;
     };
-    s_seek();
-    // scores of the step at the S cursor, one step ahead of the products
+    // scores of the step at the S cursor
     auto issue_s = [&]() -> bool {
       if (s_j == 0 && !wait(q_full, s_items & 1, 34)) return false;
       const uint32_t ks = s_g % S::kStages;
@@ -494,14 +498,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       if (++s_j == s_it.steps) {
         ++s_items;
         s_j = 0;
-        s_seek();
+        s_more = false;
       }
       return true;
     };
-    ok = ok && (!s_more || issue_s());
-    while (take()) {
+    // Scores of the steps before `limit`. Those of step g have to be under way before its product; where P lies beside S those
+    // of step g + 1 too, otherwise these follow the product, which reads P where they go.
+    auto scores_to = [&](uint32_t limit) {
+      while (ok && s_g < limit && s_seek()) ok = issue_s();
+    };
+    for (s_seek(); take(); s_seek()) {
       for (int j = 0; j < it.steps && ok; ++j, ++g) {
-        if (S::kAhead && s_more && !(ok = issue_s())) break;
+        scores_to(g + (S::kAhead ? 2 : 1));
+        if (!ok) break;
         const uint32_t vs = g % S::kStages, ph = (g / S::kStages) & 1;
         const bool active = j < it.blocks(h);
         if (active && !(ok = wait(&p_full[h], n & 1, 37))) break;
@@ -520,7 +529,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         }
         __syncwarp();
         n += active;
-        if (!S::kAhead && s_more) ok = issue_s();
+        if (!S::kAhead) scores_to(g + 2);
       }
     }
     }

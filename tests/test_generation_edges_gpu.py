@@ -1,0 +1,49 @@
+"""The attention over the paged cache where numbers and plans go to extremes, against the plain form in 64 bits."""
+import pytest
+import torch
+
+from generation import Plan, attention_64, attention_bound, new_cache
+from pequegrad_b200 import kernels as K
+from test_generation_gpu import attend, check, randn, same
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, I8 = torch.float16, torch.bfloat16, torch.int8
+
+# new tokens, contexts, heads: tiles of sixteen rows; chunks whose keys are split over a cluster; chunks that are not split
+SIZES = [([2, 3], [400, 700], 2), ([200], [700], 2), ([40] * 24, [520] * 24, 8)]
+
+
+def check_numbers(plan, q, cache, got):
+    """What is a number in the plain form is one, within the bound; the rest is NaN in both."""
+    D = q.shape[-1]
+    want, mass, size = attention_64(plan, q, cache, D ** -0.5)
+    nan = want.isnan()
+    assert torch.equal(got.isnan(), nan), f"{int(got.isnan().sum())} NaN for {int(nan.sum())}"
+    mass = mass.nan_to_num(0)
+    bound = attention_bound(want, mass, size, q.dtype, D, max(plan.ctx), float(mass.max()) * 4 + 1)
+    err = (got.double() - want).abs()
+    assert bool((err <= bound)[~nan].all()), float((err - bound)[~nan].max())
+    assert K.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype,cache,D", [(F16, F16, 64), (BF16, BF16, 128), (F16, I8, 64), (BF16, I8, 128)])
+@pytest.mark.parametrize("new,ctx", [([20] * 50, [0] * 50), ([300] * 20 + [20] * 30, [-5] * 50), ([100] * 24 + [20] * 60, [300] * 24 + [0] * 60), ([150] * 12 + [1] * 90, [260] * 12 + [0] * 90)])
+def test_hundreds_of_work_items_without_a_key(new, ctx, dtype, cache, D):
+    # several in a row for every CTA, alone and behind items with keys; with a table and without one
+    H = 12
+    plan = Plan(new, ctx, 32, pad_rows=2)
+    c = new_cache(plan, H, D, cache)
+    q = randn(plan.rows, H, D, dtype=dtype)
+    outs = []
+    for table in [plan.table] + ([plan.table[:, :0]] if max(ctx) <= 0 else []):
+        out = torch.full_like(q, 7)
+        plan.table = table
+        attend(plan, q, c, out=out)
+        check(plan, out, q, c)
+        for b, n in enumerate(ctx):
+            if n <= 0:
+                assert (out[plan.starts[b]:plan.starts[b + 1]] == 0).all()
+        assert (out[-2:] == 7).all()
+        outs.append(out)
+    assert same(outs[0], attend(plan, q, c, out=torch.full_like(q, 7)))
