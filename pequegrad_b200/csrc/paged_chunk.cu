@@ -49,7 +49,7 @@ namespace pgb {
 
 constexpr int kChunkRows = 256;     // of an item
 constexpr int kChunkThreads = 512;
-constexpr uint32_t kChunkPolls = 1u << 20;
+constexpr uint32_t kChunkPolls = 1u << 20;  // eight seconds, when nothing comes
 constexpr float kChunkLazy = 8.0f;  // log2 of the largest probability before a row's reference moves
 constexpr int kScaleSlots = 4;
 constexpr int kItemSlots = 4;  // items found ahead
@@ -257,6 +257,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
   int *dead = const_cast<int *>(abort_flag) + 1;
   volatile int *poison = const_cast<volatile int *>(abort_flag) + 2;
+  volatile uint32_t *moved = tmem_slot + 4;  // [half] steps whose products were issued
 
   // broadcast, so that the compiler knows it is the same for the warp: barrier addresses and descriptors stay uniform
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -292,6 +293,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     }
     *abort_flag = 0;
     *poison = 0;
+    moved[0] = moved[1] = 0;
     *dead = *(volatile int *)P.err != 0;  // an earlier wait ran out and nobody has cleared the word: do nothing
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -338,7 +340,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     }
   };
   // Some wait for a whole item, which a context of 2^30 tokens makes seconds long. Each ends when a role that waits for one
-  // step at a time ends, or gives up and raises the flag that every wait looks at.
+  // step at a time gives up, or the role that finds the items sees nothing move, and raises the flag that every wait looks at.
   const uint32_t patient = P.polls < (1u << 20) ? P.polls : 1u << 31;
   // a wait of the whole warp; `role` goes into the error word
   auto wait = [&](uint64_t *bar, uint32_t parity, int role, uint32_t polls = 0) -> bool {
@@ -422,11 +424,21 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
   if (!run) {
   } else if (warp >= 12) {
     if (warp == 15) {
+      // Waits until every reader has given a slot up. While it waits here, other roles may be waiting for items or whole items
+      // of Q: it ends that wait, for all of them, when no product was issued during a full count of polls.
+      auto given_up = [&](uint32_t slot, uint32_t parity) -> bool {
+        for (uint32_t seen = ~0u;;) {
+          const uint32_t now = __shfl_sync(0xffffffffu, moved[0] + moved[1], 0);
+          if (now == seen) return wait(&item_empty[slot], parity, 47, 1);
+          seen = now;
+          if (__all_sync(0xffffffffu, attn_wait(&item_empty[slot], parity, abort_flag, P.polls))) return true;
+        }
+      };
       for (bool more = true; more && ok; ++taken) {
         const int id = id_of((int)taken);
         more = id < n_items && chunk_item(P, id, rank, cur, it);
-        const uint32_t slot = taken % kItemSlots;
-        if (!(ok = wait(&item_empty[slot], ((taken / kItemSlots) & 1) ^ 1, 47, patient))) break;
+        const uint32_t slot = taken % kItemSlots, parity = (taken / kItemSlots) & 1;
+        if (!(ok = given_up(slot, parity ^ 1))) break;
         if (lane == 0) {
           item_s[4 * slot] = make_int4(more ? it.seq : -1, it.head, it.token, it.sub);
           item_s[4 * slot + 1] = make_int4(it.rows, it.pos, it.n_keys, it.first_seen);
@@ -434,6 +446,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
           mbar_arrive(&item_full[slot]);
         }
         __syncwarp();
+        if (!more || P.splits > 1) ok = given_up(slot, parity);  // the last of all items, or of this round: nobody waits for one after it
         if (P.splits > 1) {  // one between two joins
           ++taken;
           break;
@@ -526,6 +539,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
           } else {
             mbar_arrive(&v_empty[vs]);
           }
+          moved[h] = g;
         }
         __syncwarp();
         n += active;

@@ -47,3 +47,17 @@ def test_hundreds_of_work_items_without_a_key(new, ctx, dtype, cache, D):
         assert (out[-2:] == 7).all()
         outs.append(out)
     assert same(outs[0], attend(plan, q, c, out=torch.full_like(q, 7)))
+
+
+@pytest.mark.parametrize("cache", [F16, I8])
+def test_waits_for_items_end_with_the_others(cache):
+    # a launch that loads nothing and whose first items have no keys: roles that wait for items give up when nothing moves
+    plan = Plan([20] * 60 + [200] * 4, [0] * 60 + [200] * 4, 32)
+    c = new_cache(plan, 12, 64, cache)
+    q = randn(plan.rows, 12, 64)
+    K.gemm_wait_drill(1 << 14, skip_loads=True)
+    attend(plan, q, c)
+    torch.cuda.synchronize()
+    code = K.device_error(reset=True)
+    assert 32 <= code >> 16 <= 47
+    check(plan, attend(plan, q, c), q, c)

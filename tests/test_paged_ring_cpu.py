@@ -53,6 +53,7 @@ class Cta:
             yield self.item_empty[i % SLOTS], ((i // SLOTS) & 1) ^ 1
             self.slot[i % SLOTS] = (i, item)
             self.item_full[i % SLOTS].arrive()
+        yield self.item_empty[i % SLOTS], (i // SLOTS) & 1  # until every reader knows that there are no more
 
     def queries(self):
         taken = n = 0
@@ -156,7 +157,8 @@ class Cta:
 
     def run(self, rng):
         """True if every role came to its end."""
-        roles = [self.finder(), self.queries(), self.keys(), self.softmax(0), self.softmax(1), self.products_of(0), self.products_of(1)]
+        finder = self.finder()
+        roles = [finder, self.queries(), self.keys(), self.softmax(0), self.softmax(1), self.products_of(0), self.products_of(1)]
         at = {r: None for r in roles}
         while at:
             moved = False
@@ -169,6 +171,7 @@ class Cta:
                     except StopIteration:
                         del at[r]
             if not moved:
+                assert finder in at, "nobody sees that nothing moves"
                 return False
         return True
 
@@ -185,7 +188,7 @@ def item(rng, none):
 @pytest.mark.parametrize("stages,beside", [(3, True), (2, True), (2, False), (1, False)])
 @pytest.mark.parametrize("masked", [False, True])
 def test_every_order_of_items_comes_to_its_end(stages, beside, masked):
-    for seed in range(150):
+    for seed in range(60):
         rng = random.Random(seed)
         none = rng.choice([0.0, 0.2, 0.5, 0.9, 1.0])
         items = [item(rng, none) for _ in range(rng.randint(0, 30))]
