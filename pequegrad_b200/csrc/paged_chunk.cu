@@ -935,12 +935,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
   __syncthreads();
   if (run && *abort_flag != 0 && !gone) {
     // Some role gave up. Copies and products that are in flight are waited for, with a limit again: nothing may write the
-    // memory of a CTA that has gone.
+    // memory of a CTA that has gone. The roles that did not give up have to stop too: in a cluster there are rounds to come, and
+    // what they would start there nobody sees out.
     gone = true;
+    ok = false;
     auto see_out = [&](uint64_t *bar, uint32_t parity) {
       for (uint32_t i = 0; i < kChunkPolls && !mbar_try_wait(bar, parity); ++i) {}
     };
-    if (!I8 && warp == 8) {
+    if (warp < 8) {
+      tmem_ld_wait();
+      tmem_st_wait();
+    } else if (!I8 && warp == 8) {
       for (uint32_t st = 0; st < S::kStages; ++st) {
         if (s_n > st) see_out(&k_full[(s_n - 1 - st) % S::kStages], ((s_n - 1 - st) / S::kStages) & 1);
         if (n > st) see_out(&v_full[(n - 1 - st) % S::kStages], ((n - 1 - st) / S::kStages) & 1);

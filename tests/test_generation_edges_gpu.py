@@ -61,3 +61,24 @@ def test_waits_for_items_end_with_the_others(cache):
     code = K.device_error(reset=True)
     assert 32 <= code >> 16 <= 47
     check(plan, attend(plan, q, c), q, c)
+
+
+@pytest.mark.parametrize("dtype,cache,D", [(F16, F16, 64), (BF16, BF16, 128), (F16, I8, 64)])
+@pytest.mark.parametrize("new,ctx,H", [([200], [6000], 60), ([300] * 10, [400] * 10, 40)])
+def test_waits_cut_short_leave_nothing_behind(new, ctx, H, dtype, cache, D):
+    """Waits of so few polls run out in the middle of the work, or do not, in clusters with several rounds to go and outside. A
+    launch that gave up says so, and the next one is right."""
+    plan = Plan(new, ctx, 64)
+    c = new_cache(plan, H, D, cache)
+    q = randn(plan.rows, H, D, dtype=dtype)
+    for polls in (1, 2, 8):
+        K.gemm_wait_drill(polls, skip_loads=False)
+        out = attend(plan, q, c)
+        torch.cuda.synchronize()
+        code = K.device_error(reset=True)
+        assert code == 0 or 32 <= code >> 16 <= 47
+        right = attend(plan, q, c)
+        if polls == 1:
+            check(plan, right, q, c)
+            first = right
+        assert same(right, first) and (code != 0 or same(out, first))
