@@ -684,8 +684,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       // last key that this row sees, and the warp's first row; rows that do not exist see what the last one does
       const int lim = last_seen(it, row);
       const int warp_lim = __shfl_sync(0xffffffffu, lim, 0);
-      float m = -INFINITY, l = 0.f, lv = 0.f;  // reference of the exponents: m * c + lv, lv = log2 of the value scales' power of two
-      bool have_lv = false;
+      // Reference of the exponents: m * c + lv, lv = log2 of the value scales' power of two. It begins at a scale whose values
+      // are nothing in fp16, so that zero scales alone have a reference too.
+      float m = -INFINITY, l = 0.f, lv = I8 && HALF ? -40.f : 0.f;
       auto page_of = [&](int j) -> int {  // of this lane's sixteen keys of step j; looked up a step early, used when it is there
         const int i = (((it.lo + j) << 7) + 16 * (lane & 7)) >> P.c.log2_page;
         return j < it.steps && (i << P.c.log2_page) < it.n_keys ? __ldg(P.p.table + (int64_t)it.seq * P.p.pitch + i) : 0;
@@ -773,10 +774,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
           const float4 t4 = *reinterpret_cast<const float4 *>(sc + 256);
           const uint32_t e = __float_as_uint(fmaxf(fmaxf(t4.x, t4.y), fmaxf(t4.z, t4.w))) >> 23;
           const float lv_blk = (float)(int)e - 127.f;
-          if (e > 0 && e < 255 && (!have_lv || lv_blk > lv)) {
-            shift += have_lv ? lv - lv_blk : 0.f;
+          if (e < 255 && lv_blk > lv) {
+            shift += lv - lv_blk;
             lv = lv_blk;
-            have_lv = true;
           }
         }
         const float alpha = shift == 0.f ? 1.f : ex2f(shift);

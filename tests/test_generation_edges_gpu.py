@@ -82,3 +82,18 @@ def test_waits_cut_short_leave_nothing_behind(new, ctx, H, dtype, cache, D):
             check(plan, right, q, c)
             first = right
         assert same(right, first) and (code != 0 or same(out, first))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new,ctx,H", SIZES)
+@pytest.mark.parametrize("zeros", [128, 300])
+def test_values_of_scale_zero_have_their_share_of_the_softmax(dtype, D, new, ctx, H, zeros):
+    # whole blocks of keys whose values are zeros, stored with a scale of zero, before ordinary ones
+    plan = Plan(new, ctx, 32)
+    c = new_cache(plan, H, D, I8)
+    for b in range(len(new)):
+        for page, slot in plan.places(b, range(zeros)):
+            c[3][page, :, slot] = 0
+    q = randn(plan.rows, H, D, dtype=dtype)
+    check(plan, attend(plan, q, c), q, c)
