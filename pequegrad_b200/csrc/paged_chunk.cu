@@ -762,8 +762,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         }
         if (I8 || masked) tmem_st_wait();
         tmem_ld32_issue(s_addr, x0);
-        // A score that is no number makes the row's sum none either. (It would be lost in the polynomial of the exponentials.)
-        if (mx != mx) l = mx;
+        // A score that is no number makes the row's sum none either, and so does +infinity, whose exponent is infinity less itself.
+        // (Both would be lost in the polynomial of the exponentials.)
+        if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);
         const float m_cand = fmaxf(m, mx);
         const bool grow = (m_cand - m) * c > kChunkLazy;  // -inf -> finite: true; -inf -> -inf is NaN: false
         const float m_new = grow ? m_cand : m;

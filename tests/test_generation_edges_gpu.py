@@ -97,3 +97,20 @@ def test_values_of_scale_zero_have_their_share_of_the_softmax(dtype, D, new, ctx
             c[3][page, :, slot] = 0
     q = randn(plan.rows, H, D, dtype=dtype)
     check(plan, attend(plan, q, c), q, c)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new,ctx,H", SIZES)
+def test_an_infinite_key(dtype, D, new, ctx, H):
+    """Every second row has a score of +infinity, and with it no softmax; for the others that score is -infinity and the key
+    does not count. At each place in eight neighbours, in a block that all rows see and in one that only some do."""
+    plan = Plan(new, ctx, 32)
+    q = randn(plan.rows, H, D, dtype=dtype)
+    q[::2, 0, 3], q[1::2, 0, 3] = 1, -1
+    clean = new_cache(plan, H, D, dtype)
+    for at in [*range(136, 144), *range(ctx[0] - 8, ctx[0])]:
+        c = (clean[0].clone(), *clean[1:])
+        page, slot = plan.places(0, [at])[0]
+        c[0][page, 0, slot, 3] = float("inf")
+        check_numbers(plan, q, c, attend(plan, q, c))
