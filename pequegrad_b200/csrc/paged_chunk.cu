@@ -687,6 +687,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       // Reference of the exponents: m * c + lv, lv = log2 of the value scales' power of two. It begins at a scale whose values
       // are nothing in fp16, so that zero scales alone have a reference too.
       float m = -INFINITY, l = 0.f, lv = I8 && HALF ? -40.f : 0.f;
+      uint32_t met = 0;  // not zero: the row has a key
       auto page_of = [&](int j) -> int {  // of this lane's sixteen keys of step j; looked up a step early, used when it is there
         const int i = (((it.lo + j) << 7) + 16 * (lane & 7)) >> P.c.log2_page;
         return j < it.steps && (i << P.c.log2_page) < it.n_keys ? __ldg(P.p.table + (int64_t)it.seq * P.p.pitch + i) : 0;
@@ -736,6 +737,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
             uint32_t keep = more >= 31 ? 0xffffffffu : more < 0 ? 0u : (2u << more) - 1;
             if ((absent >> (c >> 4)) & 1) keep &= 0xffff0000u;
             if ((absent >> (c >> 4)) & 2) keep &= 0xffffu;
+            met |= keep;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (!((keep >> i) & 1)) x[i] = 0xff800000u;  // -inf
@@ -762,6 +764,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         }
         if (I8 || masked) tmem_st_wait();
         tmem_ld32_issue(s_addr, x0);
+        if (!masked) met = 1;
         // A score that is no number makes the row's sum none either, and so does +infinity, whose exponent is infinity less itself.
         // (Both would be lost in the polynomial of the exponentials.)
         if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);
@@ -905,19 +908,21 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         if (!ok) continue;
         tc_fence_after();
       }
-      const bool seen = any && !(l == 0.f);  // the row met a key (a score that is no number leaves l no number either)
+      // No key, or none with a score above -infinity: then the softmax is that of nothing (zeros) or no number. A part of a split
+      // item says which in its sum, and nobody reads its O. (A score that is NaN leaves l NaN.)
+      const bool low = m == -INFINITY && l == l;
       if (P.splits > 1) {  // joined below
-        ml_s[row] = seen ? (m == -INFINITY ? 0.f : m * c) + lv : -INFINITY;
-        ml_s[kChunkRows + row] = l;
+        ml_s[row] = low ? -INFINITY : (m == -INFINITY ? 0.f : m * c) + lv;
+        ml_s[kChunkRows + row] = low ? (met ? 1.f : 0.f) : l;
         continue;
       }
-      const float inv = seen ? 1.0f / l : 0.f;
+      const float inv = low ? (met ? __uint_as_float(0x7fc00000u) : 0.f) : 1.0f / l;
       const bool slow = !I8 && any && *poison != 0;
       uint8_t *out = out_row(it, row);
 #pragma unroll 1
       for (int q = 0; q < D / 32; ++q) {
         float o[32];
-        load_o(it, o_addr, q, any, seen, slow, lim, o);
+        load_o(it, o_addr, q, any, !low, slow, lim, o);
         if (row < it.rows) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -1015,7 +1020,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         sum += pl[s] * e;
         if (s == part) mine = e;
       }
-      weight[part * kShare + row] = mm == -INFINITY ? 0.f : mine / sum;
+      if (mm == -INFINITY) {  // no part has a score above that: zeros without a key, else no number
+        float keys = 0.f;
+#pragma unroll
+        for (int s = 0; s < N; ++s) keys += pl[s];
+        mine = keys > 0.f ? __uint_as_float(0x7fc00000u) : 0.f;
+        sum = 1.f;
+      }
+      weight[part * kShare + row] = mine / sum;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < n_rows * kParts; i += kChunkThreads) {

@@ -239,6 +239,7 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
   // Reference of the exponents: m + lv. lv is the power of two of the value scales met so far: the scaled probabilities then
   // stay within fp16, and since it is the same for all rows and in the sums too, O / l is what it was.
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, lv = I8 ? -100.f : 0.f;
+  bool met[2] = {false, false};  // the row has a key
 
   Entries pages[S::kStages];  // table entries of the blocks under way
 #pragma unroll
@@ -306,11 +307,13 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
           for (int e = 0; e < 4; ++e) {
             const int key = key0 + 16 * u + 8 * h + 2 * t + (e & 1);
             if (key > lim[e >> 1] || absent[u]) s[u][h][e] = -INFINITY;
+            else met[e >> 1] = true;
             // a slot behind the context has a stale scale: its probability of zero must meet a number
             if (I8 && e < 2 && (key >= n_keys || absent[u])) vs[u][2 * h + e] = 0.f;
           }
       }
     }
+    if (!masked) met[0] = met[1] = true;
     float mx[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -432,6 +435,7 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
   for (int r = 0; r < 2; ++r) {
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    met[r] = (__ballot_sync(0xffffffffu, met[r]) >> (lane & 28)) & 15;
   }
   __syncthreads();  // every warp is done with its stages: the memory now holds partial results
 
@@ -452,8 +456,11 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
         dst[d + kCol * (2 * t + 1)] = o[i][2 * r + 1];
       }
       if (t == 0) {
-        part_m[warp * 16 + row] = m[r] == -INFINITY && !(l[r] == 0.f) ? 0.f : m[r] + lv;  // a score that is no number: so is l
-        part_l[warp * 16 + row] = l[r];
+        // No key, or none with a score above -infinity: the sum says which, and the softmax is that of nothing (zeros) or no number.
+        // With a score that is NaN, so is l.
+        const bool low = m[r] == -INFINITY && l[r] == 0.f;
+        part_m[warp * 16 + row] = low ? -INFINITY : (m[r] == -INFINITY ? 0.f : m[r] + lv);
+        part_l[warp * 16 + row] = low ? (met[r] ? 1.f : 0.f) : l[r];
       }
     }
   }
@@ -479,9 +486,12 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
         x += part[(w * 16 + row) * D + d] * e;
         sum += part_l[w * 16 + row] * e;
       }
+    } else {
+#pragma unroll
+      for (int w = 0; w < kRowWarps; ++w) sum += part_l[w * 16 + row];
     }
     if (splits == 1) {
-      write(row, d, mm == -INFINITY ? 0.f : x / sum);
+      write(row, d, mm == -INFINITY ? (sum == 0.f ? 0.f : NAN) : x / sum);
     } else {
       mine[row * D + d] = x;
       if (d == 0) { mine_m[row] = mm; mine_l[row] = sum; }
@@ -502,8 +512,10 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
         x += ld_cluster(at + 4 * i, s) * e;
         sum += ld_cluster(at_l + 4 * row, s) * e;
       }
+    } else {
+      for (int s = 0; s < splits; ++s) sum += ld_cluster(at_l + 4 * row, s);
     }
-    write(row, d, mm == -INFINITY ? 0.f : x / sum);
+    write(row, d, mm == -INFINITY ? (sum == 0.f ? 0.f : NAN) : x / sum);
   }
   cluster_sync();  // nobody's shared memory goes away while it is read
 }

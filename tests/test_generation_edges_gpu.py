@@ -114,3 +114,20 @@ def test_an_infinite_key(dtype, D, new, ctx, H):
         page, slot = plan.places(0, [at])[0]
         c[0][page, 0, slot, 3] = float("inf")
         check_numbers(plan, q, c, attend(plan, q, c))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new,ctx,H", SIZES + [([1], [1], 2), ([150], [150], 2)])
+def test_rows_whose_every_score_is_minus_infinity(dtype, D, new, ctx, H):
+    """They have keys, so they are not rows without one: minus infinity less itself is NaN in the plain softmax. Head 1 is
+    left alone; in head 0 all keys are infinite, or those of the first 200 positions, which then do not count."""
+    plan = Plan(new, ctx, 32)
+    q = randn(plan.rows, H, D, dtype=dtype)
+    q[:, 0, 3] = -1
+    for first in (max(ctx), 200):
+        c = new_cache(plan, H, D, dtype)
+        for b, n in enumerate(ctx):
+            for page, slot in plan.places(b, range(min(first, n))):
+                c[0][page, 0, slot, 3] = float("inf")
+        check_numbers(plan, q, c, attend(plan, q, c))
