@@ -19,8 +19,8 @@
 // Tensor memory: S_A [0, 128), S_B [128, 256), O_A, O_B behind them. With head dim 64 there is room for P beside S, and the
 // scores of the next block are computed under the softmax of this one; with 128 P takes the place of S, and the two halves
 // keep the tensor pipe and the exponentials busy in turn.
-// int8 scales: the key's multiplies its scores, the value's its probabilities, both in fp32. In fp16 the product's range is
-// kept by a common power of two per block, which joins the exponents' reference and leaves O / l as it is.
+// int8 scales: the key's multiplies its scores, the value's its probabilities, both in fp32. In fp16 the products' range is
+// kept by a reference of the exponents that counts the value scale's power of two, row by row; O / l is what it was.
 // Masked places: a score that is left out is -inf by selection, its probability zero. Value rows behind the context are
 // zeroed in shared memory, and values of new tokens that some rows must not see are cleared of NaN and infinities there;
 // the rows that do see such a token get them back in the epilogue.
@@ -51,6 +51,9 @@ constexpr int kChunkRows = 256;     // of an item
 constexpr int kChunkThreads = 512;
 constexpr uint32_t kChunkPolls = 1u << 20;  // eight seconds, when nothing comes
 constexpr float kChunkLazy = 8.0f;  // log2 of the largest probability before a row's reference moves
+// log2 of the smallest value scale that has a say in fp16 outputs: 127 times less is nothing there. With it zero scales have an
+// exponent, and a row's sum stays within fp32.
+constexpr float kChunkNothing = -40.0f;
 constexpr int kScaleSlots = 4;
 constexpr int kItemSlots = 4;  // items found ahead
 constexpr int kItemReaders = 15;  // warps that read them: all but the one that finds them
@@ -62,7 +65,7 @@ struct ChunkTile {
   static constexpr int kStages = I8 ? (D == 64 ? 2 : 1) : (D == 64 ? 3 : 2);
   static constexpr int kRawStages = I8 ? (D == 64 ? 3 : 2) : 0;
   static constexpr int kRing = 2 * kStages * kKV + kRawStages * kRaw;
-  static constexpr int kScales = I8 ? kScaleSlots * (2 * 128 + 4) * 4 : 0;
+  static constexpr int kScales = I8 ? kScaleSlots * 3 * 128 * 4 : 0;
   static constexpr int kMl = 3 * kChunkRows * 4;  // m and l of the rows, weights of the parts
   static constexpr int kSmem = kQ + kRing + kScales + kMl + kItemSlots * 64 + 512 /*barriers*/ + 1024 /*alignment*/;
   static_assert(kRing >= kChunkRows * D * 4, "the partial results of a split item take the place of the rings");
@@ -244,7 +247,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
   uint8_t *k_s = q_s + S::kQ;                   // [stage][d / 64][128 keys][128 bytes]
   uint8_t *v_s = k_s + S::kStages * S::kKV;
   uint8_t *raw_s = v_s + S::kStages * S::kKV;   // [stage][K, V][128 keys][D bytes]
-  float *scale_s = reinterpret_cast<float *>(raw_s + S::kRawStages * S::kRaw);  // [slot][128 of K, 128 of V, 4 maxima]
+  float *scale_s = reinterpret_cast<float *>(raw_s + S::kRawStages * S::kRaw);  // [slot][128 of K, 128 of V, 128 exponents of V's]
   float *ml_s = scale_s + S::kScales / 4;       // [m, l][256], [part][rows that this CTA writes]
   int4 *item_s = reinterpret_cast<int4 *>(ml_s + 3 * kChunkRows);  // [slot][4]
   uint64_t *bars = reinterpret_cast<uint64_t *>(item_s + 4 * kItemSlots);
@@ -651,13 +654,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
           __syncwarp();
           if (lane == 0) mbar_arrive(&k_full[st]);
           if (!(ok = wait(&sc_empty[slot], ((g / kScaleSlots) & 1) ^ 1, 40))) break;
-          float *sc = scale_s + slot * (2 * 128 + 4);
+          float *sc = scale_s + slot * (3 * 128);
           sc[key] = ks[0];
           sc[128 + key] = vs[0];
-          float top = fabsf(vs[0]);
-#pragma unroll
-          for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-          if (lane == 0) sc[256 + w] = top;
+          const int e = (int)((__float_as_uint(vs[0]) >> 23) & 255);
+          sc[256 + key] = e == 255 ? kChunkNothing : fmaxf((float)(e - 127), kChunkNothing);
           __syncwarp();
           if (lane == 0) mbar_arrive(&sc_full[slot]);
           if (!(ok = wait(&v_empty[st], ph, 33))) break;
@@ -684,9 +685,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       // last key that this row sees, and the warp's first row; rows that do not exist see what the last one does
       const int lim = last_seen(it, row);
       const int warp_lim = __shfl_sync(0xffffffffu, lim, 0);
-      // Reference of the exponents: m * c + lv, lv = log2 of the value scales' power of two. It begins at a scale whose values
-      // are nothing in fp16, so that zero scales alone have a reference too.
-      float m = -INFINITY, l = 0.f, lv = I8 && HALF ? -40.f : 0.f;
+      float m = -INFINITY, l = 0.f;  // reference of the exponents, and the sum of their powers
       uint32_t met = 0;  // not zero: the row has a key
       auto page_of = [&](int j) -> int {  // of this lane's sixteen keys of step j; looked up a step early, used when it is there
         const int i = (((it.lo + j) << 7) + 16 * (lane & 7)) >> P.c.log2_page;
@@ -717,7 +716,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         const int key0 = (it.lo + j) << 7;
         const bool masked = key0 + 127 > warp_lim || absent != 0;  // warp-uniform
         const int last = lim - key0;                               // last of the 128 that the row sees
-        const float *sc = scale_s + slot * (2 * 128 + 4);
+        const float *sc = scale_s + slot * (3 * 128);
+        // The largest exponent. Beside an int8 cache the probabilities take their values' scales with them into 16 bits: with fp16 it
+        // is then the largest of the products that counts, each score with its value scale's power of two. Whatever ratios the scales
+        // have, and wherever the tokens are that a row does not see, the largest product is of order one.
+        constexpr bool kProducts = I8 && HALF;
         float mx = -INFINITY;
         // The first pass scales int8 scores by their keys and puts -inf where the row must not look; it writes what it changed
         // back, so that the second pass takes every score as it finds it.
@@ -746,10 +749,21 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
           float mq[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            mq[q] = max3_nan(__uint_as_float(x[8 * q]), __uint_as_float(x[8 * q + 1]), __uint_as_float(x[8 * q + 2]));
-            mq[q] = max3_nan(mq[q], __uint_as_float(x[8 * q + 3]), __uint_as_float(x[8 * q + 4]));
-            mq[q] = max3_nan(mq[q], __uint_as_float(x[8 * q + 5]), __uint_as_float(x[8 * q + 6]));
-            mq[q] = max3_nan(mq[q], mq[q], __uint_as_float(x[8 * q + 7]));
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+              float4 z = make_float4(__uint_as_float(x[8 * q + i]), __uint_as_float(x[8 * q + i + 1]), __uint_as_float(x[8 * q + i + 2]), __uint_as_float(x[8 * q + i + 3]));
+              if (kProducts) {
+                const float4 e4 = *reinterpret_cast<const float4 *>(sc + 256 + c + 8 * q + i);
+                const float2 u = fma2(make_float2(z.x, z.y), c2, make_float2(e4.x, e4.y)), v = fma2(make_float2(z.z, z.w), c2, make_float2(e4.z, e4.w));
+                z = make_float4(u.x, u.y, v.x, v.y);
+              }
+              y[i] = z.x; y[i + 1] = z.y; y[i + 2] = z.z; y[i + 3] = z.w;
+            }
+            mq[q] = max3_nan(y[0], y[1], y[2]);
+            mq[q] = max3_nan(mq[q], y[3], y[4]);
+            mq[q] = max3_nan(mq[q], y[5], y[6]);
+            mq[q] = max3_nan(mq[q], mq[q], y[7]);
           }
           mx = max3_nan(mx, max3_nan(mq[0], mq[1], mq[2]), mq[3]);
         };
@@ -765,26 +779,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         if (I8 || masked) tmem_st_wait();
         tmem_ld32_issue(s_addr, x0);
         if (!masked) met = 1;
+        if (!kProducts) mx *= c;
         // A score that is no number makes the row's sum none either, and so does +infinity, whose exponent is infinity less itself.
         // (Both would be lost in the polynomial of the exponentials.)
         if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);
         const float m_cand = fmaxf(m, mx);
-        const bool grow = (m_cand - m) * c > kChunkLazy;  // -inf -> finite: true; -inf -> -inf is NaN: false
+        const bool grow = m_cand - m > kChunkLazy;  // -inf -> finite: true; -inf -> -inf is NaN: false
         const float m_new = grow ? m_cand : m;
         const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        float shift = grow ? (m - m_use) * c : 0.f;
-        if constexpr (I8 && HALF) {
-          // probabilities times value scales stay within fp16: the largest scale's power of two joins the reference
-          const float4 t4 = *reinterpret_cast<const float4 *>(sc + 256);
-          const uint32_t e = __float_as_uint(fmaxf(fmaxf(t4.x, t4.y), fmaxf(t4.z, t4.w))) >> 23;
-          const float lv_blk = (float)(int)e - 127.f;
-          if (e < 255 && lv_blk > lv) {
-            shift += lv - lv_blk;
-            lv = lv_blk;
-          }
-        }
-        const float alpha = shift == 0.f ? 1.f : ex2f(shift);
-        const float nmc = -m_use * c - lv;
+        const float alpha = grow ? ex2f(m - m_use) : 1.f;
+        const float nmc = -m_use;
         const float2 nmc2 = make_float2(nmc, nmc);
         m = m_new;
         if (n > 0) {
@@ -912,7 +916,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       // item says which in its sum, and nobody reads its O. (A score that is NaN leaves l NaN.)
       const bool low = m == -INFINITY && l == l;
       if (P.splits > 1) {  // joined below
-        ml_s[row] = low ? -INFINITY : (m == -INFINITY ? 0.f : m * c) + lv;
+        ml_s[row] = low || m != -INFINITY ? m : 0.f;
         ml_s[kChunkRows + row] = low ? (met ? 1.f : 0.f) : l;
         continue;
       }

@@ -236,9 +236,11 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
   float o[D / 8][4];
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  // Reference of the exponents: m + lv. lv is the power of two of the value scales met so far: the scaled probabilities then
-  // stay within fp16, and since it is the same for all rows and in the sums too, O / l is what it was.
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, lv = I8 ? -100.f : 0.f;
+  // m is the reference of the exponents. Beside an int8 cache it counts the power of two of each key's value scale: the scaled
+  // probabilities then stay within fp16, the largest of a row at order one, whatever ratios the scales have and whatever
+  // lies where the row must not look. It is in the sums too, so O / l is what it was.
+  constexpr float kNothing = -100.f;  // log2 of a scale whose values are nothing: a sum of 2^100s is within fp32
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   bool met[2] = {false, false};  // the row has a key
 
   Entries pages[S::kStages];  // table entries of the blocks under way
@@ -314,40 +316,42 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
       }
     }
     if (!masked) met[0] = met[1] = true;
-    float mx[2];
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float ev = 0.f;
+          if constexpr (I8) {
+            const int top = (int)((__float_as_uint(vs[u][2 * h + e]) >> 23) & 255);
+            ev = top == 255 ? kNothing : fmaxf((float)(top - 127), kNothing);
+          }
+          mx[0] = fmaxf(mx[0], I8 ? s[u][h][e] + ev : s[u][h][e]);
+          mx[1] = fmaxf(mx[1], I8 ? s[u][h][2 + e] + ev : s[u][h][2 + e]);
+        }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      mx[r] = fmaxf(fmaxf(s[0][0][2 * r], s[0][0][2 * r + 1]), fmaxf(s[0][1][2 * r], s[0][1][2 * r + 1]));
-      if (U == 2) mx[r] = fmaxf(mx[r], fmaxf(fmaxf(s[U - 1][0][2 * r], s[U - 1][0][2 * r + 1]), fmaxf(s[U - 1][1][2 * r], s[U - 1][1][2 * r + 1])));
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
     }
-    float lv_new = lv;
-    if constexpr (I8) {
-      float top = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[0][2], vs[0][3]));
-      if (U == 2) top = fmaxf(top, fmaxf(fmaxf(vs[U - 1][0], vs[U - 1][1]), fmaxf(vs[U - 1][2], vs[U - 1][3])));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const uint32_t e = __float_as_uint(top) >> 23;
-      if (e < 255) lv_new = fmaxf(lv, (float)(int)e - 127.f);
-    }
-    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1] || lv_new != lv)) {  // rare once the largest scores have been met
+    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {  // rare once the largest scores have been met
       float alpha[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const float mn = fmaxf(m[r], mx[r]);
-        alpha[r] = mn == -INFINITY ? 1.f : paged_ex2(m[r] - mn + (lv - lv_new));
+        alpha[r] = mn == -INFINITY ? 1.f : paged_ex2(m[r] - mn);
         m[r] = mn;
         l[r] *= alpha[r];
       }
-      lv = lv_new;
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) {
         o[i][0] *= alpha[0]; o[i][1] *= alpha[0];
         o[i][2] *= alpha[1]; o[i][3] *= alpha[1];
       }
     }
-    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0] + lv, m[1] == -INFINITY ? 0.f : m[1] + lv};
+    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
     bool cleared = false;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -459,7 +463,7 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
         // No key, or none with a score above -infinity: the sum says which, and the softmax is that of nothing (zeros) or no number.
         // With a score that is NaN, so is l.
         const bool low = m[r] == -INFINITY && l[r] == 0.f;
-        part_m[warp * 16 + row] = low ? -INFINITY : (m[r] == -INFINITY ? 0.f : m[r] + lv);
+        part_m[warp * 16 + row] = low || m[r] != -INFINITY ? m[r] : 0.f;
         part_l[warp * 16 + row] = low ? (met[r] ? 1.f : 0.f) : l[r];
       }
     }

@@ -131,3 +131,31 @@ def test_rows_whose_every_score_is_minus_infinity(dtype, D, new, ctx, H):
             for page, slot in plan.places(b, range(min(first, n))):
                 c[0][page, 0, slot, 3] = float("inf")
         check_numbers(plan, q, c, attend(plan, q, c))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new,ctx,H", SIZES)
+@pytest.mark.parametrize("where", ["early", "last"])
+def test_value_scales_of_any_ratio(dtype, D, new, ctx, H, where):
+    """One token's values are 2^26 times the others', and nobody looks at it: it lies 60 below the other scores, or it is the
+    last token, which only one row sees. What the others give must not be rounded away beside it.
+
+    Probabilities times value scales are rounded to fp16 relative to the row's largest such product, P >= 1 of its scale: what
+    is below 2^-25 of it is dropped. The key that has it also has a value of at least 64 of the 127 among its 64 or more, so
+    each key loses at most 2^-25 * 127 <= 2^-24 of the row's largest sum of |p v|."""
+    plan = Plan(new, ctx, 32)
+    c = new_cache(plan, H, D, I8)
+    c[3].mul_(2.0 ** -12)
+    q = randn(plan.rows, H, D, dtype=dtype).abs() + 0.5
+    for b, n in enumerate(ctx):
+        page, slot = plan.places(b, [150 if where == "early" else n - 1])[0]
+        c[3][page, :, slot] = 2.0 ** 8
+        if where == "early":
+            c[0][page, :, slot], c[2][page, :, slot] = -127, 0.1
+    got = attend(plan, q, c)
+    want, mass, size = attention_64(plan, q, c, D ** -0.5)
+    bound = attention_bound(want, mass, size, dtype, D, 0, 0.0) + max(ctx) * 2.0 ** -24 * mass.amax(-1, keepdim=True)
+    err = (got.double() - want).abs()
+    assert bool((err <= bound).all()), (float((err - bound).max()), float((err / mass).max()))
+    assert K.device_error() == 0
