@@ -37,8 +37,8 @@ static int parse_pages(const char *what, const char *name, const pgb_tensor &t, 
   for (int d = 0; d < 3; ++d) {
     if (t.stride_bytes[d] < 0 || t.stride_bytes[d] % 16)
       return fail(PGB_ERR_UNSUPPORTED, what, std::string(name) + " must have page, head and slot pitches that are multiples of 16 bytes");
-    if (writes && t.shape[d] > 1 && t.stride_bytes[d] < t.shape[3] * es) return fail(PGB_ERR_INVALID_ARG, what, std::string(name) + " overlaps itself");
   }
+  if (writes && view_overlaps_itself(view_of(t, es))) return fail(PGB_ERR_INVALID_ARG, what, std::string(name) + " overlaps itself");
   p.base = static_cast<uint8_t *>(t.data);
   p.page = t.stride_bytes[0];
   p.head = t.stride_bytes[1];
@@ -51,7 +51,7 @@ static int parse_pages(const char *what, const char *name, const pgb_tensor &t, 
   if (scale->stride_bytes[2] != 4 || scale->stride_bytes[0] < 0 || scale->stride_bytes[1] < 0 || scale->stride_bytes[0] % 16 ||
       scale->stride_bytes[1] % 16 || (reinterpret_cast<uintptr_t>(scale->data) & 15))
     return fail(PGB_ERR_UNSUPPORTED, what, "the scales of a page must be contiguous and 16-byte aligned");
-  if (writes && ((scale->shape[0] > 1 && scale->stride_bytes[0] < 4 * t.shape[2]) || (scale->shape[1] > 1 && scale->stride_bytes[1] < 4 * t.shape[2])))
+  if (writes && view_overlaps_itself(view_of(*scale, 4)))
     return fail(PGB_ERR_INVALID_ARG, what, "the scales overlap themselves");
   if (!scale->data && t.shape[0]) return fail(PGB_ERR_INVALID_ARG, what, "null scales");
   p.scale = static_cast<float *>(scale->data);
@@ -124,7 +124,7 @@ int kv_parse_rows(const char *what, const char *name, const pgb_tensor *t, int64
   if ((reinterpret_cast<uintptr_t>(t->data) & 15) || t->stride_bytes[0] < 0 || t->stride_bytes[1] < 0 ||
       (t->shape[0] > 1 && t->stride_bytes[0] % 16) || (heads > 1 && t->stride_bytes[1] % 16))
     return fail(PGB_ERR_UNSUPPORTED, what, std::string(name) + " must be 16-byte aligned with row and head pitches that are multiples of 16 bytes");
-  if (writes && ((t->shape[0] > 1 && t->stride_bytes[0] < head_dim * es) || (heads > 1 && t->stride_bytes[1] < head_dim * es)))
+  if (writes && view_overlaps_itself(view_of(*t, es)))
     return fail(PGB_ERR_INVALID_ARG, what, std::string(name) + " overlaps itself");
   if (t->shape[0] > 2147483647LL) return fail(PGB_ERR_UNSUPPORTED, what, "too many rows");
   if (t->shape[0] && !t->data) return fail(PGB_ERR_INVALID_ARG, what, std::string("null ") + name);

@@ -6,6 +6,7 @@
 #include <string>
 
 #include "gemm.hpp"
+#include "overlap.hpp"
 #include "reduce_common.cuh"
 
 namespace pgb {
