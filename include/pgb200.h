@@ -389,7 +389,10 @@ PGB_API int pgb_peer_allgather(const void *src, size_t bytes, void *const *peer_
  *   page_table  int32 [sequences, n]: entry i is the page of positions i * page size and up. A position outside the table,
  *               or an entry outside 0 .. pages - 1 (-1, say), has no page.
  * They are read on the device. Rows behind the last sequence are padding: they are neither read for their values nor
- * written. A plan can say nothing that makes a kernel reach outside the tensors it was given. */
+ * written. A plan can say nothing that makes a kernel reach outside the tensors it was given.
+ *
+ * What these calls write must not overlap itself, and shares no memory with anything else that the call is given, but for
+ * what is said below. */
 
 /* Stores new rows: k, v [rows, heads, head dim] (f16 or bf16, views with a contiguous head dim and 16-byte pitches). Into a
  * 16-bit cache (of their dtype) they are copied; into an int8 cache each token's head is quantised by the rule of
@@ -412,7 +415,7 @@ PGB_API int pgb_kv_read(const pgb_tensor *k_cache, const pgb_tensor *v_cache, co
  *   q, out   [rows, q heads, head dim] f16 or bf16, views with a contiguous head dim and 16-byte pitches; q heads is a
  *            multiple of the cache's heads, and consecutive query heads share a key head
  *   cache    of q's dtype, or int8
- * A row without a key gets zeros. One token per sequence or a long chunk, mixed as they come. fp32 accumulation and softmax
+ * A row without a key gets zeros. `out` may be q itself. One token per sequence or a long chunk, mixed as they come. fp32 accumulation and softmax
  * statistics. */
 PGB_API int pgb_paged_attention(const pgb_tensor *q, const pgb_tensor *k_cache, const pgb_tensor *v_cache,
                                 const pgb_tensor *k_scale, const pgb_tensor *v_scale, const pgb_tensor *q_start,
@@ -427,7 +430,7 @@ PGB_API int pgb_paged_attention(const pgb_tensor *q, const pgb_tensor *k_cache, 
  *   out[r, v] = bit v % 32 of mask[r, v / 32] set ? x : -inf
  * Each part may be NULL: history [rows, n] int32 (then no penalties, lengths); history_len, prompt_len int32 [rows] (n and
  * 0); repetition, frequency, presence f32 [rows] (1, 0, 0); bias_ids int32 and bias f32 [rows, m]; mask int32 [rows, words].
- * Token ids outside the vocabulary are passed over. out may be logits itself. The vocabulary dim is contiguous, rows at
+ * Token ids outside the vocabulary are passed over. out may be logits itself, but no other view of it. The vocabulary dim is contiguous, rows at
  * any pitch. */
 PGB_API int pgb_logits_process(const pgb_tensor *logits, const pgb_tensor *history, const pgb_tensor *history_len,
                                const pgb_tensor *prompt_len, const pgb_tensor *repetition, const pgb_tensor *frequency,

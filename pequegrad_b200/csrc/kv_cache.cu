@@ -133,6 +133,30 @@ int kv_parse_rows(const char *what, const char *name, const pgb_tensor *t, int64
   return PGB_OK;
 }
 
+int kv_apart(const char *what, std::initializer_list<KvOperand> written, std::initializer_list<KvOperand> read) {
+  ByteView w[4];  // the cache's two tensors and their scales at most
+  int n = 0;
+  const KvOperand *of[4];
+  auto alone = [&](const KvOperand &o, const ByteView &v) -> bool {
+    for (int i = 0; i < n; ++i)
+      if (views_share(w[i], v)) {
+        set_error(std::string(what) + ": " + of[i]->name + " is written and shares memory with " + o.name);
+        return false;
+      }
+    return true;
+  };
+  for (const KvOperand &o : written) {
+    if (!o.t) continue;
+    const ByteView v = view_of(*o.t, dtype_size(o.t->dtype));
+    if (!alone(o, v)) return PGB_ERR_INVALID_ARG;
+    w[n] = v;
+    of[n++] = &o;
+  }
+  for (const KvOperand &o : read)
+    if (o.t && !alone(o, view_of(*o.t, dtype_size(o.t->dtype)))) return PGB_ERR_INVALID_ARG;
+  return PGB_OK;
+}
+
 struct KvRows {
   uint8_t *k, *v;
   int64_t k_row, k_head, v_row, v_head;  // bytes
@@ -336,6 +360,9 @@ static int kv_write(const pgb_tensor *k, const pgb_tensor *v, const pgb_tensor *
   x.v = static_cast<uint8_t *>(v->data);
   x.rows = k->shape[0];
   if (!kv_device_present()) return PGB_ERR_CUDA;
+  if ((st = kv_apart(what, {{"k_cache", k_cache}, {"v_cache", v_cache}, {"k_scale", k_scale}, {"v_scale", v_scale}},
+                     {{"k", k}, {"v", v}, {"q_start", q_start}, {"ctx_len", ctx_len}, {"page_table", page_table}})) != PGB_OK)
+    return st;
   if (x.rows == 0 || p.n_seq == 0 || c.n_pages == 0 || p.width == 0) return PGB_OK;
   const int64_t grid = (x.rows * c.heads * (c.head_dim / 8) + 255) / 256;
   if (grid > 2147483647LL) return fail(PGB_ERR_UNSUPPORTED, what, "too many rows");
@@ -375,6 +402,9 @@ static int kv_read(const pgb_tensor *k_cache, const pgb_tensor *v_cache, const p
   y.v = static_cast<uint8_t *>(v->data);
   y.rows = k->shape[0];
   if (!kv_device_present()) return PGB_ERR_CUDA;
+  if ((st = kv_apart(what, {{"k", k}, {"v", v}},
+                     {{"k_cache", k_cache}, {"v_cache", v_cache}, {"k_scale", k_scale}, {"v_scale", v_scale}, {"kv_start", kv_start}, {"page_table", page_table}})) != PGB_OK)
+    return st;
   if (y.rows == 0 || p.n_seq == 0) return PGB_OK;
   const int lanes = i8 ? c.head_dim / 16 : c.head_dim / 8;
   const int64_t grid = (y.rows * c.heads * lanes + 255) / 256;

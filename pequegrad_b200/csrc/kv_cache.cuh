@@ -3,6 +3,7 @@
 //
 // The reference's GPT-2 recomputes every position for each new token (examples/gpt2.py:406-438) and has no cache.
 #pragma once
+#include <initializer_list>
 #include <string>
 
 #include "gemm.hpp"
@@ -69,5 +70,11 @@ int kv_parse_plan(const char *what, const pgb_tensor *start, const pgb_tensor *c
 int kv_parse_rows(const char *what, const char *name, const pgb_tensor *t, int64_t heads, int head_dim, bool writes, int64_t *row,
                   int64_t *head);
 bool kv_device_present();
+// No tensor of `written` may share memory with another one or with one of `read`: null tensors are passed over.
+struct KvOperand {
+  const char *name;
+  const pgb_tensor *t;
+};
+int kv_apart(const char *what, std::initializer_list<KvOperand> written, std::initializer_list<KvOperand> read);
 
 }  // namespace pgb

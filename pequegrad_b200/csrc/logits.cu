@@ -16,6 +16,7 @@
 #include <cstring>
 #include <string>
 
+#include "overlap.hpp"
 #include "reduce_common.cuh"
 #include "vec.cuh"
 
@@ -274,6 +275,13 @@ static int logits_process(const pgb_tensor *logits, const pgb_tensor *history, c
     return PGB_ERR_CUDA;
   }
   if (rows == 0 || V == 0) return PGB_OK;
+  const ByteView written = view_of(*out, es);
+  for (const pgb_tensor *t : {logits, history, history_len, prompt_len, repetition, frequency, presence, bias_ids, bias, mask}) {
+    if (!t) continue;
+    const ByteView v = view_of(*t, dtype_size(t->dtype));
+    if (views_share(written, v) && !(t == logits && v == written))
+      return bad(PGB_ERR_INVALID_ARG, "out shares memory with an operand (it may be logits itself, but no other view of it)");
+  }
   p.x = logits->data;
   p.y = out->data;
   p.V = V;

@@ -38,6 +38,12 @@ static int paged_attention(const pgb_tensor *q, const pgb_tensor *k_cache, const
   if ((st = kv_parse_rows(what, "out", out, H, c.head_dim, true, &a.o_row, &a.o_head)) != PGB_OK) return st;
   if (out->shape[0] != q->shape[0]) return fail(PGB_ERR_INVALID_ARG, "q and out differ in rows");
   if (!kv_device_present()) return PGB_ERR_CUDA;
+  // A row's queries are read before its result is written, and by nobody else: out may be q.
+  const bool in_place = view_of(*out, 2) == view_of(*q, 2);
+  if ((st = kv_apart(what, {{"out", out}},
+                     {{"q", in_place ? nullptr : q}, {"k_cache", k_cache}, {"v_cache", v_cache}, {"k_scale", k_scale}, {"v_scale", v_scale},
+                      {"q_start", q_start}, {"ctx_len", ctx_len}, {"page_table", page_table}})) != PGB_OK)
+    return st;
   a.q = static_cast<const uint8_t *>(q->data);
   a.out = static_cast<uint8_t *>(out->data);
   a.rows = q->shape[0];

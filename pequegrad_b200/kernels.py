@@ -338,7 +338,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     v_scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of new rows q [rows, query heads, D] over their sequences' cached keys and values (their own among
     them: `kv_write` comes first). The plan is the one of `kv_write`; rows without a key get zeros, rows behind the last
-    sequence are not written."""
+    sequence are not written. `out` may be `q`."""
     if scale is None:
         scale = float(q.shape[-1]) ** -0.5
     if out is None:

@@ -159,3 +159,56 @@ def test_value_scales_of_any_ratio(dtype, D, new, ctx, H, where):
     err = (got.double() - want).abs()
     assert bool((err <= bound).all()), (float((err - bound).max()), float((err / mass).max()))
     assert K.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype,cache,D,Hq,Hkv", [(F16, F16, 64, 4, 4), (BF16, BF16, 128, 8, 2), (F16, I8, 128, 6, 2), (BF16, I8, 64, 20, 1)])
+@pytest.mark.parametrize("new,ctx", [([1, 3, 0, 2], [700, 40, 9, 2000]), ([200, 1, 64], [700, 5, 90]), ([90] * 30, [300] * 30)])
+def test_the_result_may_take_the_queries_place(new, ctx, dtype, cache, D, Hq, Hkv):
+    plan = Plan(new, ctx, 32, pad_rows=2)
+    c = new_cache(plan, Hkv, D, cache)
+    qkv = randn(plan.rows, Hq + 2 * Hkv, D, dtype=dtype)
+    keep = qkv.clone()
+    want = attend(plan, keep[:, :Hq], c, out=keep[:, :Hq].clone())
+    assert attend(plan, qkv[:, :Hq], c, out=qkv[:, :Hq]) is not None
+    assert same(qkv[:, :Hq], want) and same(qkv[:, Hq:], keep[:, Hq:])
+
+
+def test_results_that_share_memory_are_refused():
+    H, D, P = 2, 64, 16
+    plan = Plan([5, 3], [20, 9], P)
+    n = plan.kv_starts[-1]
+    kc, vc, _, _ = new_cache(plan, H, D, F16)
+    k8, v8, ks, vs = new_cache(plan, H, D, I8)
+    at = (plan.q_start, plan.ctx_len, plan.table)
+    buf = randn(n + 1, 3, H, D)
+    keep = [x.clone() for x in (kc, vc, buf, ks, vs)]
+
+    def refused(call, *names):
+        with pytest.raises(Exception, match="shares memory") as e:
+            call()
+        assert all(name in str(e.value) for name in names), str(e.value)
+
+    x = buf[:plan.rows]
+    refused(lambda: K.kv_write(x[:, 0], x[:, 1], kc, kc, *at), "v_cache", "k_cache")
+    refused(lambda: K.kv_write(x[:, 0], x[:, 1], kc[1:], kc[:-1], *at), "v_cache", "k_cache")
+    refused(lambda: K.kv_write(x[:, 0], x[:, 1], k8, v8, *at, ks, ks), "k_scale", "v_scale")
+    refused(lambda: K.kv_write(kc.view(-1, H, D)[3:3 + plan.rows], x[:, 1], kc, vc, *at), "k_cache")
+    refused(lambda: K.kv_read(kc, vc, plan.kv_start, plan.table, n, out=(buf[:n, 0], buf[:n, 0])), "k", "v")
+    refused(lambda: K.kv_read(kc, vc, plan.kv_start, plan.table, n, out=(buf[:n, 0], buf[1:, 0])), "k", "v")
+    refused(lambda: K.kv_read(kc, vc, plan.kv_start, plan.table, 2, out=(buf[:2, 0], vc.view(-1, H, D)[:2])), "v_cache")
+    refused(lambda: K.paged_attention(x[:, 0], kc, vc, *at, out=x.flatten(1, 2)[:, 1:1 + H]), "out", "q")
+    refused(lambda: K.paged_attention(buf[:plan.rows, 0], kc, vc, *at, out=buf[1:plan.rows + 1, 0]), "out", "q")
+    refused(lambda: K.paged_attention(x[:, 0], kc, vc, *at, out=vc.view(-1, H, D)[:plan.rows]), "v_cache")
+    rows = torch.randn((4, 40), device="cuda")
+    refused(lambda: K.logits_process(rows[:, :30], out=rows[:, 1:31]))
+    refused(lambda: K.logits_process(rows[:3], out=rows[1:]))
+    refused(lambda: K.logits_process(rows, bias_ids=torch.zeros((4, 2), dtype=torch.int32, device="cuda"), bias=rows[:, :2], out=rows))
+    for a, b in zip((kc, vc, buf, ks, vs), keep):
+        assert same(a, b)
+    # neighbours in one buffer are apart
+    K.kv_read(kc, vc, plan.kv_start, plan.table, n, out=(buf[:n, 0], buf[:n, 2]))
+    both = torch.zeros((plan.pages, 2, H, P, D), dtype=F16, device="cuda")
+    K.kv_write(x[:, 0], x[:, 1], both[:, 0], both[:, 1], *at)
+    K.paged_attention(x[:, 0], kc, vc, *at, out=x[:, 1])
+    K.logits_process(rows[:, :20], out=rows[:, 20:])
+    torch.cuda.synchronize()
