@@ -218,9 +218,10 @@ static int bad(int status, const std::string &msg) {
   return status;
 }
 
-// An optional [rows] or [rows, n] operand of 32-bit values whose rows are contiguous.
+// An optional [rows] or [rows, n] operand of 32-bit values whose rows are contiguous. Only one without values may be null.
 static bool rows_of(const pgb_tensor *t, int dtype, int ndim, int64_t rows, int64_t *n, int64_t *pitch) {
   if (t->dtype != dtype || t->ndim != ndim || t->shape[0] != rows || (reinterpret_cast<uintptr_t>(t->data) & 3)) return false;
+  if (rows > 0 && (ndim == 1 || t->shape[1] > 0) && !t->data) return false;
   if (ndim == 1) return rows <= 1 || t->stride_bytes[0] == 4;
   if ((t->shape[1] > 1 && t->stride_bytes[1] != 4) || t->stride_bytes[0] < 0 || t->stride_bytes[0] % 4) return false;
   *n = t->shape[1];
@@ -240,6 +241,7 @@ static int logits_process(const pgb_tensor *logits, const pgb_tensor *history, c
   if (logits->ndim != 2 || out->ndim != 2 || logits->shape[0] != out->shape[0] || logits->shape[1] != out->shape[1] || out->dtype != logits->dtype)
     return bad(PGB_ERR_INVALID_ARG, "logits and out must be [rows, vocabulary] of one dtype");
   const int64_t rows = logits->shape[0], V = logits->shape[1];
+  if (rows && V && (!logits->data || !out->data)) return bad(PGB_ERR_INVALID_ARG, "null tensor");
   for (const pgb_tensor *t : {logits, out})
     if ((V > 1 && t->stride_bytes[1] != es) || t->stride_bytes[0] < 0 || t->stride_bytes[0] % es || (reinterpret_cast<uintptr_t>(t->data) & (es - 1)))
       return bad(PGB_ERR_INVALID_ARG, "the vocabulary dim must be contiguous");
