@@ -97,7 +97,7 @@ int kv_parse_plan(const char *what, const pgb_tensor *start, const pgb_tensor *c
   if (start->ndim != 1 || start->shape[0] < 1 || !is_contiguous(*start)) return fail(PGB_ERR_INVALID_ARG, what, "the row offsets must be a contiguous [sequences + 1]");
   const int64_t B = start->shape[0] - 1;
   if (ctx && (ctx->ndim != 1 || ctx->shape[0] != B || !is_contiguous(*ctx))) return fail(PGB_ERR_INVALID_ARG, what, "the lengths must be a contiguous [sequences]");
-  if (table->ndim != 2 || table->shape[0] != B) return fail(PGB_ERR_INVALID_ARG, what, "the page table must be [sequences, pages of a sequence]");
+  if (table->ndim != 2 || table->shape[0] != B || table->shape[1] < 0) return fail(PGB_ERR_INVALID_ARG, what, "the page table must be [sequences, pages of a sequence]");
   if (table->shape[1] > 1 && table->stride_bytes[1] != 4) return fail(PGB_ERR_INVALID_ARG, what, "the rows of the page table must be contiguous");
   if (table->stride_bytes[0] < 0 || table->stride_bytes[0] % 4) return fail(PGB_ERR_INVALID_ARG, what, "bad stride in the page table");
   // positions are 32-bit numbers: 2^23 pages of at most 128 tokens
@@ -126,6 +126,7 @@ int kv_parse_rows(const char *what, const char *name, const pgb_tensor *t, int64
     return fail(PGB_ERR_UNSUPPORTED, what, std::string(name) + " must be 16-byte aligned with row and head pitches that are multiples of 16 bytes");
   if (writes && view_overlaps_itself(view_of(*t, es)))
     return fail(PGB_ERR_INVALID_ARG, what, std::string(name) + " overlaps itself");
+  if (t->shape[0] < 0) return fail(PGB_ERR_INVALID_ARG, what, std::string(name) + " has a negative number of rows");
   if (t->shape[0] > 2147483647LL) return fail(PGB_ERR_UNSUPPORTED, what, "too many rows");
   if (t->shape[0] && !t->data) return fail(PGB_ERR_INVALID_ARG, what, std::string("null ") + name);
   *row = t->shape[0] > 1 ? t->stride_bytes[0] : 0;

@@ -223,7 +223,7 @@ static bool rows_of(const pgb_tensor *t, int dtype, int ndim, int64_t rows, int6
   if (t->dtype != dtype || t->ndim != ndim || t->shape[0] != rows || (reinterpret_cast<uintptr_t>(t->data) & 3)) return false;
   if (rows > 0 && (ndim == 1 || t->shape[1] > 0) && !t->data) return false;
   if (ndim == 1) return rows <= 1 || t->stride_bytes[0] == 4;
-  if ((t->shape[1] > 1 && t->stride_bytes[1] != 4) || t->stride_bytes[0] < 0 || t->stride_bytes[0] % 4) return false;
+  if (t->shape[1] < 0 || (t->shape[1] > 1 && t->stride_bytes[1] != 4) || t->stride_bytes[0] < 0 || t->stride_bytes[0] % 4) return false;
   *n = t->shape[1];
   *pitch = t->stride_bytes[0] / 4;
   return true;
@@ -241,6 +241,7 @@ static int logits_process(const pgb_tensor *logits, const pgb_tensor *history, c
   if (logits->ndim != 2 || out->ndim != 2 || logits->shape[0] != out->shape[0] || logits->shape[1] != out->shape[1] || out->dtype != logits->dtype)
     return bad(PGB_ERR_INVALID_ARG, "logits and out must be [rows, vocabulary] of one dtype");
   const int64_t rows = logits->shape[0], V = logits->shape[1];
+  if (rows < 0 || V < 0) return bad(PGB_ERR_INVALID_ARG, "negative rows or vocabulary");
   if (rows && V && (!logits->data || !out->data)) return bad(PGB_ERR_INVALID_ARG, "null tensor");
   for (const pgb_tensor *t : {logits, out})
     if ((V > 1 && t->stride_bytes[1] != es) || t->stride_bytes[0] < 0 || t->stride_bytes[0] % es || (reinterpret_cast<uintptr_t>(t->data) & (es - 1)))
@@ -250,7 +251,7 @@ static int logits_process(const pgb_tensor *logits, const pgb_tensor *history, c
   LogitParams p{};
   int64_t n = 0;
   if (history) {
-    if (!rows_of(history, PGB_I32, 2, rows, &n, &p.history_pitch) || n > 2147483647LL) return bad(PGB_ERR_INVALID_ARG, "history must be int32 [rows, tokens]");
+    if (!rows_of(history, PGB_I32, 2, rows, &n, &p.history_pitch) || n > 2147483647LL - 65536) return bad(PGB_ERR_INVALID_ARG, "history must be int32 [rows, tokens]");
     p.L = (int)n;
   } else if (history_len || prompt_len || repetition || frequency || presence) {
     return bad(PGB_ERR_INVALID_ARG, "penalties and lengths need a history");

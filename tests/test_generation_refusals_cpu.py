@@ -1,6 +1,6 @@
-"""Calls of generation that a C caller can make and that must not reach the device: null data."""
+"""Calls of generation that a C caller can make and that must not reach the device: null data, extents below zero."""
 from pequegrad_b200 import _lib as L
-from test_generation_cpu import i32, logits, refused, t
+from test_generation_cpu import CACHE, attend, i32, logits, read, refused, t, write
 
 bad = L.ERR_INVALID_ARG
 
@@ -18,3 +18,17 @@ def test_null_data_of_logits_and_their_operands():
     refused(logits(ids=i32(3, 2, ptr=0), bias=t((3, 2), L.F32)), bad, b"[rows, entries]")
     refused(logits(ids=i32(3, 2), bias=f32(3, 2)), bad, b"[rows, entries]")
     refused(logits(mask=i32(3, 4, ptr=0)), bad, b"a bit for each")
+
+
+def test_extents_below_zero():
+    s = (256, 64, 1)
+    refused(write(k=t((-5, 4, 64), strides=s), v=t((-5, 4, 64), strides=s)), bad, b"negative number of rows")
+    refused(read(k=t((-5, 4, 64), strides=s), v=t((-5, 4, 64), strides=s)), bad, b"negative number of rows")
+    refused(attend(q=t((-5, 8, 64), strides=(512, 64, 1)), out=t((-5, 8, 64), strides=(512, 64, 1))), bad, b"negative number of rows")
+    for call in (write, read, attend):
+        refused(call(table=i32(3, -7, strides=(7, 1))), bad, b"page table must be")
+        refused(call(kc=t((-9, *CACHE[1:]), strides=(8192, 2048, 64, 1)), vc=t((-9, *CACHE[1:]), strides=(8192, 2048, 64, 1))), L.ERR_UNSUPPORTED, b"bad number of pages")
+    refused(logits(x=t((-3, 100), strides=(100, 1)), out=t((-3, 100), strides=(100, 1))), bad, b"negative rows")
+    refused(logits(x=t((3, -100), strides=(100, 1)), out=t((3, -100), strides=(100, 1))), bad, b"negative rows")
+    refused(logits(history=i32(3, -9, strides=(9, 1))), bad, b"history must be")
+    refused(logits(ids=i32(3, -2, strides=(2, 1)), bias=t((3, -2), L.F32, strides=(2, 1))), bad, b"[rows, entries]")
