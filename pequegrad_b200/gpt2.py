@@ -117,6 +117,8 @@ class GPT2:
         D = C // H
         if ids.shape != (R,):
             raise ValueError("GPT2.forward_cached: one token id per row of the plan")
+        if last_only and plan.fewest == 0:
+            raise ValueError("GPT2.forward_cached: a sequence without a new token has no last row")
         if plan.longest > cfg.block_size:
             raise ValueError("GPT2.forward_cached: a sequence is longer than block_size")
         tok, pos = K.embedding_rows(ids, self.wte, None, 1), K.embedding_rows(plan.positions, self.wpe, None, 1)

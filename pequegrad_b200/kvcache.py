@@ -16,8 +16,8 @@ from . import kernels as K
 
 class KVPlan:
     """One step of some sequences: row offsets, lengths and page table on the device (see `kernels.kv_write`), and the
-    position of every row. `rows` is their number, `last` the row of each sequence's last new token, `longest` the longest
-    context."""
+    position of every row. `rows` is their number, `last` the row of each sequence's last new token (-1 without one), `fewest` the
+    smallest number of new tokens of a sequence, `longest` the longest context."""
 
     def __init__(self, new: Sequence[int], ctx: Sequence[int], tables: Sequence[Sequence[int]], device):
         start = [0]
@@ -25,12 +25,12 @@ class KVPlan:
             start.append(start[-1] + n)
         width = max((len(t) for t in tables), default=0)
         # one upload: offsets, lengths, last rows, positions, table
-        flat = start + list(ctx) + [s - 1 for s in start[1:]]
+        flat = start + list(ctx) + [s - 1 if n else -1 for s, n in zip(start[1:], new)]
         for n, c in zip(new, ctx):
             flat.extend(range(c - n, c))
         for t in tables:
             flat.extend(list(t) + [-1] * (width - len(t)))
-        B, self.rows, self.longest = len(new), start[-1], max(ctx, default=0)
+        B, self.rows, self.longest, self.fewest = len(new), start[-1], max(ctx, default=0), min(new, default=1)
         dev = torch.tensor(flat, dtype=torch.int32).to(device)
         at = 0
 
