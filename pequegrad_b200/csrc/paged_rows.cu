@@ -563,11 +563,15 @@ static int launch(const PagedParams &a, const KvCache &c, const KvPlan &p, int s
 int run_paged_rows(const PagedParams &a, const KvCache &c, const KvPlan &p, bool half, cudaStream_t stream) {
   const int tiles_per_token = (a.group + 15) / 16;
   const int64_t units = a.rows * tiles_per_token * c.heads;
+  // A row that begins no tile has CTAs too, which return at once: it is the tiles that count below, of which each sequence that
+  // has rows adds at most one that is not full.
+  const int64_t tokens = a.group >= 16 ? 1 : 16 / a.group, k = p.n_seq < a.rows ? p.n_seq : a.rows;
+  const int64_t tiles = ((a.rows - k) / tokens + k) * tiles_per_token * c.heads;
   // As many CTAs per item as leave no SM idle, up to a portable cluster; not more than have a block of keys for each warp.
   int splits = 1;
   const int warps = c.head_dim == 64 ? 2 : 4;
   const int64_t blocks = ((int64_t)p.width << c.log2_page) / (c.head_dim == 64 ? 32 : 16);
-  while (splits < 8 && units * splits < 4LL * sm_count() && blocks > (int64_t)splits * warps) splits *= 2;
+  while (splits < 8 && tiles * splits < 4LL * sm_count() && blocks > (int64_t)splits * warps) splits *= 2;
   if (units * splits > 2147483647LL) {
     set_error("paged_attention: too many rows for one launch");
     return PGB_ERR_UNSUPPORTED;

@@ -212,3 +212,16 @@ def test_results_that_share_memory_are_refused():
     K.paged_attention(x[:, 0], kc, vc, *at, out=x[:, 1])
     K.logits_process(rows[:, :20], out=rows[:, 20:])
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype,cache,D,Hq,Hkv", [(F16, F16, 64, 12, 12), (BF16, BF16, 128, 16, 16), (F16, I8, 128, 6, 2), (BF16, I8, 64, 15, 5), (F16, F16, 128, 18, 1)])
+@pytest.mark.parametrize("new,ctx", [([5] * 4, [3000] * 4), ([2, 4, 1, 3], [2500, 31, 700, 4000]), ([5, 5], [129, 128])])
+def test_a_few_tokens_over_long_contexts(new, ctx, dtype, cache, D, Hq, Hkv):
+    # rows that begin no tile beside clusters whose keys are split as far as they go
+    plan = Plan(new, ctx, 64, pad_rows=3)
+    c = new_cache(plan, Hkv, D, cache)
+    q = randn(plan.rows, Hq, D, dtype=dtype)
+    out = torch.full_like(q, 7)
+    attend(plan, q, c, out=out)
+    check(plan, out, q, c)
+    assert (out[plan.starts[-1]:] == 7).all() and same(out[:plan.starts[-1]], attend(plan, q, c)[:plan.starts[-1]])
