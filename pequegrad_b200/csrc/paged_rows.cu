@@ -12,9 +12,9 @@
 //   softmax  running maximum and sum per row in fp32; the warps' and then the CTAs' partial results are joined in shared and
 //            distributed shared memory, in a fixed order. No scratch in global memory, nothing shared between launches.
 //   int8     widened exactly to fp16; the key's scale multiplies its scores, the value's scale its probabilities, in fp32.
-// Measured: 16 sequences of up to 32768 int8 tokens, 32 heads of 128 on 8: 184 us, 3.3 TB/s, half the copy rate; 64 of up to
+// Measured: 16 sequences of up to 32768 int8 tokens, 32 heads of 128 on 8: 181 us, 3.4 TB/s, half the copy rate; 64 of up to
 // 1024 tokens, 12 heads of 64 in fp16: 38 us, 3.5 TB/s. What bounds them then is the latency of a warp's chain from copy to
-// second product, with the twelve warps whose registers fit an SM. Tiles of 8 rows (half the output's registers) gave 176 and
+// second product, with the twelve warps whose registers fit an SM (eight, whose stages do, with 128 values of 16 bits). Tiles of 8 rows (half the output's registers) gave 176 and
 // 39 us, a cap at 128 registers for sixteen warps 329 (spills): neither is worth a second set of kernels.
 #include <atomic>
 #include <string>
@@ -30,7 +30,6 @@ struct RowTile {
   // 64: 37 us against 41 with four); long ones: four (16 sequences of up to 32768 int8 tokens, 8 heads of 128: 184 us
   // against 191 with two and 254 with eight).
   static constexpr int kWarps = D == 64 ? 2 : 4;
-  static constexpr int kCtas = 12 / kWarps;  // resident on an SM, as registers allow
   static constexpr int kEs = I8 ? 1 : 2;
   static constexpr int kKChunks = D * kEs / 64;              // 16-byte chunks of one key that a lane holds
   static constexpr int kVBytes = D * kEs / 8;                // bytes of one value row that a lane holds
@@ -46,6 +45,8 @@ struct RowTile {
   static constexpr int kWarp = kStages * kStage;
   static constexpr int kJoin = kWarps * 16 * (D + 2) * 4;
   static constexpr int kSmem = (kWarps * kWarp > kJoin ? kWarps * kWarp : kJoin) + 16 * (D + 2) * 4;
+  static constexpr int kFit = 233472 / (kSmem + 1024);  // CTAs that the shared memory of an SM holds
+  static constexpr int kCtas = kFit < 12 / kWarps ? kFit : 12 / kWarps;  // and registers: twelve warps
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
