@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
                                                                        const __grid_constant__ ChunkParams P) {
   using S = ChunkTile<D, I8>;
   constexpr int kQWarps = I8 ? 1 : 4;  // 14 and, where keys come by TMA, 9-11
+  constexpr bool kProducts = I8 && HALF;  // the exponents' reference counts value scales too
   constexpr int kKind = GEMM_F16;  // kind::f16 serves both 16-bit types; the descriptor tells them apart
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -685,7 +686,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       // last key that this row sees, and the warp's first row; rows that do not exist see what the last one does
       const int lim = last_seen(it, row);
       const int warp_lim = __shfl_sync(0xffffffffu, lim, 0);
-      float m = -INFINITY, l = 0.f;  // reference of the exponents, and the sum of their powers
+      // Reference of the exponents, times c where it is a score, and the sum of their powers.
+      float m = -INFINITY, l = 0.f;
       uint32_t met = 0;  // not zero: the row has a key
       auto page_of = [&](int j) -> int {  // of this lane's sixteen keys of step j; looked up a step early, used when it is there
         const int i = (((it.lo + j) << 7) + 16 * (lane & 7)) >> P.c.log2_page;
@@ -720,7 +722,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         // The largest exponent. Beside an int8 cache the probabilities take their values' scales with them into 16 bits: with fp16 it
         // is then the largest of the products that counts, each score with its value scale's power of two. Whatever ratios the scales
         // have, and wherever the tokens are that a row does not see, the largest product is of order one.
-        constexpr bool kProducts = I8 && HALF;
         float mx = -INFINITY;
         // The first pass scales int8 scores by their keys and puts -inf where the row must not look; it writes what it changed
         // back, so that the second pass takes every score as it finds it.
@@ -779,16 +780,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         if (I8 || masked) tmem_st_wait();
         tmem_ld32_issue(s_addr, x0);
         if (!masked) met = 1;
-        if (!kProducts) mx *= c;
         // A score that is no number makes the row's sum none either, and so does +infinity, whose exponent is infinity less itself.
         // (Both would be lost in the polynomial of the exponentials.)
         if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);
         const float m_cand = fmaxf(m, mx);
-        const bool grow = m_cand - m > kChunkLazy;  // -inf -> finite: true; -inf -> -inf is NaN: false
+        const float unit = kProducts ? 1.f : c;  // scores are kept as they are: with exponents the step takes 3 % longer
+        const bool grow = (m_cand - m) * unit > kChunkLazy;  // -inf -> finite: true; -inf -> -inf is NaN: false
         const float m_new = grow ? m_cand : m;
         const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = grow ? ex2f(m - m_use) : 1.f;
-        const float nmc = -m_use;
+        const float alpha = grow ? ex2f((m - m_use) * unit) : 1.f;
+        const float nmc = -m_use * unit;
         const float2 nmc2 = make_float2(nmc, nmc);
         m = m_new;
         if (n > 0) {
@@ -916,7 +917,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       // item says which in its sum, and nobody reads its O. (A score that is NaN leaves l NaN.)
       const bool low = m == -INFINITY && l == l;
       if (P.splits > 1) {  // joined below
-        ml_s[row] = low || m != -INFINITY ? m : 0.f;
+        ml_s[row] = low || m != -INFINITY ? (kProducts ? m : m * c) : 0.f;
         ml_s[kChunkRows + row] = low ? (met ? 1.f : 0.f) : l;
         continue;
       }
