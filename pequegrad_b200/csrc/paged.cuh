@@ -1,6 +1,7 @@
 // Shared by the two kernels of attention over the paged cache (paged_rows.cu, paged_chunk.cu) and their entry point
 // (paged_attention.cu).
 #pragma once
+#include "attention_ptx.cuh"
 #include "kv_cache.cuh"
 
 namespace pgb {
@@ -20,17 +21,21 @@ int run_paged_rows(const PagedParams &a, const KvCache &c, const KvPlan &p, bool
 // are none: nothing was launched. Right for any number of rows.
 bool run_paged_chunk(const PagedParams &a, const KvCache &c, const KvPlan &p, bool half, cudaStream_t stream, int *status);
 
-__device__ __forceinline__ float paged_ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
+// 16 bytes into shared memory, zeros where there is nothing to copy
+__device__ __forceinline__ void paged_copy16(uint32_t dst, const void *src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-template <bool HALF>
-__device__ __forceinline__ uint32_t paged_pack(float lo, float hi) {
-  uint32_t r;
-  if (HALF) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
+// The same address in the shared memory of another CTA of the cluster
+__device__ __forceinline__ float paged_peer(uint32_t addr, uint32_t rank) {
+  uint32_t remote;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  return v;
+}
+__device__ __forceinline__ void paged_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Two of four int8 values (the low or the high pair of w) as exact 16-bit floats. fp16: the byte plus 128 is placed in the
 // mantissa of 1024, and 1152 taken off. bf16: its low seven bits in the mantissa of 128, less 128 or, where the sign bit

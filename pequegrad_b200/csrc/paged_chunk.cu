@@ -42,7 +42,6 @@
 #include <string>
 #include <type_traits>
 
-#include "attention_ptx.cuh"
 #include "paged.cuh"
 
 namespace pgb {
@@ -194,26 +193,12 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ void chunk_copy16(uint32_t dst, const void *src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ float chunk_peer(uint32_t addr, uint32_t rank) {
-  uint32_t remote;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
-  return v;
-}
 __device__ __forceinline__ float4 chunk_peer4(uint32_t addr, uint32_t rank) {
   uint32_t remote;
   float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
   return v;
-}
-__device__ __forceinline__ void chunk_cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Waits for this thread's loads from tensor memory and ties their registers to the wait.
 __device__ __forceinline__ void chunk_ld_wait(uint32_t (&v)[32]) {
@@ -413,7 +398,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         const bool in = row < it.rows;
         const uint8_t *src = P.a.q + ((int64_t)it.token + (in ? tok : 0)) * P.a.q_row + ((int64_t)it.head * P.a.group + (in ? head : 0)) * P.a.q_head + u * 16;
         const uint32_t dst = smem_u32(q_s) + (row >> 7) * (S::kQ / 2) + (u >> 3) * 16384 + (row & 127) * 128 + (((u & 7) ^ (row & 7)) << 4);
-        chunk_copy16(dst, src, in);
+        paged_copy16(dst, src, in);
         tok += step_tok;
         head += step_head;
         if (head >= P.a.group) { head -= P.a.group; ++tok; }
@@ -614,8 +599,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
               const int pg = __shfl_sync(0xffffffffu, page, kk), sl = __shfl_sync(0xffffffffu, slot, kk);
               const bool there = pg >= 0;
               const int64_t at = there ? pg : 0;
-              chunk_copy16(dst + kk * D + part * 16, P.c.k.base + at * P.c.k.page + it.head * P.c.k.head + sl * P.c.k.slot + part * 16, there);
-              chunk_copy16(dst + 128 * D + kk * D + part * 16, P.c.v.base + at * P.c.v.page + it.head * P.c.v.head + sl * P.c.v.slot + part * 16, there);
+              paged_copy16(dst + kk * D + part * 16, P.c.k.base + at * P.c.k.page + it.head * P.c.k.head + sl * P.c.k.slot + part * 16, there);
+              paged_copy16(dst + 128 * D + kk * D + part * 16, P.c.v.base + at * P.c.v.page + it.head * P.c.v.head + sl * P.c.v.slot + part * 16, there);
             }
           }
           asm volatile("cp.async.commit_group;" ::: "memory");
@@ -1002,7 +987,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     }
   }
   tc_fence_before();
-  chunk_cluster_sync();
+  paged_cluster_sync();
   // each CTA writes its share of the rows: first how much each part counts, then the weighted sums, eight values a thread
   auto join = [&](auto parts) {
     constexpr int N = decltype(parts)::value, kShare = kChunkRows / N, kParts = D / 8;
@@ -1013,8 +998,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
       float pm[N], pl[N], mm = -INFINITY, sum = 0.f;
 #pragma unroll
       for (int s = 0; s < N; ++s) {
-        pm[s] = chunk_peer(smem_u32(ml_s + r0 + row), s);
-        pl[s] = chunk_peer(smem_u32(ml_s + kChunkRows + r0 + row), s);
+        pm[s] = paged_peer(smem_u32(ml_s + r0 + row), s);
+        pl[s] = paged_peer(smem_u32(ml_s + kChunkRows + r0 + row), s);
       }
 #pragma unroll
       for (int s = 0; s < N; ++s) mm = fmaxf(mm, pm[s]);
@@ -1061,7 +1046,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
     else join(std::integral_constant<int, 8>{});
   }
   fence_proxy_async();   // TMA may write next where the partial rows lay
-  chunk_cluster_sync();  // nobody's shared memory changes or goes away while it is read
+  paged_cluster_sync();  // nobody's shared memory changes or goes away while it is read
   }
   if (warp == 12) tmem_dealloc(tmem, 512);
 }

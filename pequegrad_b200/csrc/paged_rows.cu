@@ -49,9 +49,6 @@ struct RowTile {
   static constexpr int kCtas = kFit < 12 / kWarps ? kFit : 12 / kWarps;  // and registers: twelve warps
 };
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void copy8(uint32_t dst, const void *src, bool there) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(there ? 8 : 0) : "memory");
 }
@@ -85,18 +82,6 @@ __device__ __forceinline__ uint2 ld_shared8(uint32_t a) {
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a) : "memory");
   return r;
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
-  uint32_t remote;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
-  return v;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 template <bool HALF, int D, bool I8>
 __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::kCtas) paged_rows_kernel(const __grid_constant__ PagedParams a, const __grid_constant__ KvCache c,
                                                                        const __grid_constant__ KvPlan p, unsigned splits, unsigned tiles_per_token) {
@@ -167,7 +152,7 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           uint32_t &w = q[s][2 * e + h];
-          w = paged_pack<true>(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xffff0000u) * f);
+          w = out_pair<true>(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xffff0000u) * f);
         }
     }
   }
@@ -203,7 +188,7 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
           const bool in = kWhole || quad + 8 * h < there;
 #pragma unroll
           for (int j = 0; j < S::kKChunks; ++j)
-            copy16(dst + ((h * S::kKChunks + j) * 32 + lane) * 16, in ? k + h * 8 * c.k.slot + j * 64 : c.k.base, in);
+            paged_copy16(dst + ((h * S::kKChunks + j) * 32 + lane) * 16, in ? k + h * 8 * c.k.slot + j * 64 : c.k.base, in);
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -212,7 +197,7 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
           for (int j = 0; j < S::kVPieces; ++j) {
             const uint32_t to = dst + S::kK + ((g * S::kVPieces + j) * 32 + lane) * S::kVPiece;
             const uint8_t *from = in ? v + ((g & 1) + 8 * (g >> 1)) * c.v.slot + j * 8 * S::kVPiece : c.v.base;
-            if (S::kVPiece == 16) copy16(to, from, in);
+            if (S::kVPiece == 16) paged_copy16(to, from, in);
             else copy8(to, from, in);
           }
         }
@@ -222,7 +207,7 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
       if (I8 && lane < 8) {  // scales of the block: slots are contiguous, 16 of them 16-byte aligned
         const KvPages &w = lane < 4 ? c.k : c.v;
         const float *s = w.scale + pg * w.scale_page + kvh * w.scale_head + slot0 + (lane & 3) * 4;
-        copy16(dst + S::kK + S::kV + lane * 16, s, ok);
+        paged_copy16(dst + S::kK + S::kV + lane * 16, s, ok);
       }
     }
   };
@@ -342,7 +327,7 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const float mn = fmaxf(m[r], mx[r]);
-        alpha[r] = mn == -INFINITY ? 1.f : paged_ex2(m[r] - mn);
+        alpha[r] = mn == -INFINITY ? 1.f : ex2f(m[r] - mn);
         m[r] = mn;
         l[r] *= alpha[r];
       }
@@ -362,13 +347,13 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          float x = paged_ex2(s[u][h][2 * r] - ref[r]), y = paged_ex2(s[u][h][2 * r + 1] - ref[r]);
+          float x = ex2f(s[u][h][2 * r] - ref[r]), y = ex2f(s[u][h][2 * r + 1] - ref[r]);
           l[r] += x + y;
           if (I8) {  // a token that a row does not see may have a scale that is no number
             x = x == 0.f ? 0.f : x * vs[u][2 * h];
             y = y == 0.f ? 0.f : y * vs[u][2 * h + 1];
           }
-          pa[2 * h + r] = paged_pack<kHalfMma>(x, y);
+          pa[2 * h + r] = out_pair<kHalfMma>(x, y);
         }
       const uint32_t vsrc = src + u * S::kSub + S::kK + lane * S::kVPiece;
       auto value_words = [&](int g, int j) -> uint4 {
@@ -476,7 +461,7 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
     const int tok = row / heads_here, head = row - tok * heads_here;
     uint8_t *out = a.out + (row0 + tok) * a.o_row + ((int64_t)kvh * a.group + sub * 16 + head) * a.o_head;
     const float y = __shfl_down_sync(__activemask(), x, 1);
-    if (!(d & 1)) *reinterpret_cast<uint32_t *>(out + 2 * d) = paged_pack<HALF>(x, y);
+    if (!(d & 1)) *reinterpret_cast<uint32_t *>(out + 2 * d) = out_pair<HALF>(x, y);
   };
   for (int i = threadIdx.x; i < n_rows * D; i += kRowWarps * 32) {
     const int row = i / D, d = i % D;
@@ -487,7 +472,7 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
     if (mm != -INFINITY) {
 #pragma unroll
       for (int w = 0; w < kRowWarps; ++w) {
-        const float e = paged_ex2(part_m[w * 16 + row] - mm);
+        const float e = ex2f(part_m[w * 16 + row] - mm);
         x += part[(w * 16 + row) * D + d] * e;
         sum += part_l[w * 16 + row] * e;
       }
@@ -503,26 +488,26 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
     }
   }
   if (splits == 1) return;
-  cluster_sync();
+  paged_cluster_sync();
   const uint32_t at = (uint32_t)__cvta_generic_to_shared(mine), at_m = (uint32_t)__cvta_generic_to_shared(mine_m), at_l = (uint32_t)__cvta_generic_to_shared(mine_l);
   // each CTA writes its share of the outputs: 32 of them at a time
   for (int i = (rank * kRowWarps + warp) * 32 + lane; i < n_rows * D; i += splits * kRowWarps * 32) {
     const int row = i / D, d = i % D;
     float mm = -INFINITY;
-    for (int s = 0; s < splits; ++s) mm = fmaxf(mm, ld_cluster(at_m + 4 * row, s));
+    for (int s = 0; s < splits; ++s) mm = fmaxf(mm, paged_peer(at_m + 4 * row, s));
     float x = 0.f, sum = 0.f;
     if (mm != -INFINITY) {
       for (int s = 0; s < splits; ++s) {
-        const float e = paged_ex2(ld_cluster(at_m + 4 * row, s) - mm);
-        x += ld_cluster(at + 4 * i, s) * e;
-        sum += ld_cluster(at_l + 4 * row, s) * e;
+        const float e = ex2f(paged_peer(at_m + 4 * row, s) - mm);
+        x += paged_peer(at + 4 * i, s) * e;
+        sum += paged_peer(at_l + 4 * row, s) * e;
       }
     } else {
-      for (int s = 0; s < splits; ++s) sum += ld_cluster(at_l + 4 * row, s);
+      for (int s = 0; s < splits; ++s) sum += paged_peer(at_l + 4 * row, s);
     }
     write(row, d, mm == -INFINITY ? (sum == 0.f ? 0.f : NAN) : x / sum);
   }
-  cluster_sync();  // nobody's shared memory goes away while it is read
+  paged_cluster_sync();  // nobody's shared memory goes away while it is read
 }
 
 template <bool HALF, int D, bool I8>
