@@ -226,6 +226,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
   using S = ChunkTile<D, I8>;
   constexpr int kQWarps = I8 ? 1 : 4;  // 14 and, where keys come by TMA, 9-11
   constexpr bool kProducts = I8 && HALF;  // the exponents' reference counts value scales too
+  // fp16 probabilities are held 2^7 times too large, at most 2^15 with the lag of the reference (products with value scales,
+  // which may be twice as large, 2^6): what fp16 rounds coarsely or drops is that much smaller then. The sum has the factor too.
+  constexpr float kUp = !HALF ? 0.f : kProducts ? 6.f : 7.f;
   constexpr int kKind = GEMM_F16;  // kind::f16 serves both 16-bit types; the descriptor tells them apart
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -774,7 +777,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
         const float m_new = grow ? m_cand : m;
         const float m_use = m_new == -INFINITY ? 0.f : m_new;
         const float alpha = grow ? ex2f((m - m_use) * unit) : 1.f;
-        const float nmc = -m_use * unit;
+        const float nmc = fmaf(-m_use, unit, kUp);
         const float2 nmc2 = make_float2(nmc, nmc);
         m = m_new;
         if (n > 0) {

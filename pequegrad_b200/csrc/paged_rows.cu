@@ -225,7 +225,10 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
   // m is the reference of the exponents. Beside an int8 cache it counts the power of two of each key's value scale: the scaled
   // probabilities then stay within fp16, the largest of a row at order one, whatever ratios the scales have and whatever
   // lies where the row must not look. It is in the sums too, so O / l is what it was.
-  constexpr float kNothing = -100.f;  // log2 of a scale whose values are nothing: a sum of 2^100s is within fp32
+  constexpr float kNothing = -80.f;  // log2 of a scale whose values are nothing: a sum of 2^94s is within fp32
+  // fp16 probabilities are held 2^14 times too large, at most 2^15 with a value's scale: what fp16 rounds coarsely or drops is
+  // that much smaller then. The sum has the factor too.
+  constexpr float kUp = kHalfMma ? 14.f : 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   bool met[2] = {false, false};  // the row has a key
 
@@ -337,7 +340,7 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
         o[i][2] *= alpha[1]; o[i][3] *= alpha[1];
       }
     }
-    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0] - kUp, m[1] == -INFINITY ? 0.f : m[1] - kUp};
     bool cleared = false;
 #pragma unroll
     for (int u = 0; u < U; ++u) {

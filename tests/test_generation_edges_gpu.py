@@ -225,3 +225,26 @@ def test_a_few_tokens_over_long_contexts(new, ctx, dtype, cache, D, Hq, Hkv):
     attend(plan, q, c, out=out)
     check(plan, out, q, c)
     assert (out[plan.starts[-1]:] == 7).all() and same(out[:plan.starts[-1]], attend(plan, q, c)[:plan.starts[-1]])
+
+
+@pytest.mark.parametrize("new,nats", [(1, 14.5), (1, 18.0), (3, 18.0), (40, 14.5)])
+@pytest.mark.parametrize("dtype,cache,D", [(F16, F16, 64), (F16, I8, 64), (BF16, I8, 128), (F16, F16, 128)])
+def test_many_small_probabilities_beside_one_that_is_not(new, nats, dtype, cache, D):
+    """One key lies 14.5 or 18 above 60000 others: each has a probability of 2^-21 or 2^-26, and together they make 3 % or 0.1 %
+    of the row. Probabilities are rounded to 16 bits, relative to their size as long as they are normal numbers there; nothing
+    is allowed for those that are not."""
+    H, n = 2, 60000
+    plan = Plan([new], [n], 64)
+    c = new_cache(plan, H, D, cache)
+    k = torch.zeros((n, H, D), dtype=dtype, device="cuda")
+    k[0] = nats / D ** 0.5
+    v = randn(n, H, D, dtype=dtype, seed=1).abs() + 0.5
+    v[0] = 0
+    full = Plan([n], [n], 64)
+    K.kv_write(k, v, c[0], c[1], full.q_start, full.ctx_len, plan.table, c[2], c[3])
+    q = torch.ones((new, H, D), dtype=dtype, device="cuda")
+    got = attend(plan, q, c)
+    want, mass, size = attention_64(plan, q, c, D ** -0.5)
+    err = (got.double() - want).abs()
+    bound = attention_bound(want, mass, size, dtype, D, 0, 0.0)
+    assert bool((err <= bound).all()), (float((err / want).max()), float((bound / want).max()))
