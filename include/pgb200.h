@@ -339,7 +339,7 @@ PGB_API int pgb_device_error(int *code, int reset);
 PGB_API int pgb_gemm_pair_mode(int mode);
 
 /* Failure-detection drill: the NEXT tensor-core GEMM, fused attention or chunk kernel of the paged attention launched from this host thread polls each of
- * its waits at most `polls` times and, with skip_loads != 0, its producer issues no loads, so the wait of its MMA
+ * its waits at most `polls` times (the chunk kernel's search for work again while it goes forward) and, with skip_loads != 0, its producer issues no loads, so the wait of its MMA
  * warp runs out: the kernel records the error word above, frees its tensor memory and returns; nothing faults or
  * hangs. Used by the tests to exercise the timeout path; no counterpart in the reference. */
 PGB_API int pgb_gemm_wait_drill(unsigned int polls, int skip_loads);
@@ -415,7 +415,8 @@ PGB_API int pgb_kv_read(const pgb_tensor *k_cache, const pgb_tensor *v_cache, co
  *   q, out   [rows, q heads, head dim] f16 or bf16, views with a contiguous head dim and 16-byte pitches; q heads is a
  *            multiple of the cache's heads, and consecutive query heads share a key head
  *   cache    of q's dtype, or int8
- * A row without a key gets zeros. `out` may be q itself. One token per sequence or a long chunk, mixed as they come. fp32 accumulation and softmax
+ * A row without a key gets zeros. A NaN or infinite value makes its column of the rows that see it infinite or NaN, and of
+ * no other; a NaN in a key, or a score of +infinity, the whole row NaN. `out` may be q itself. One token per sequence or a long chunk, mixed as they come. fp32 accumulation and softmax
  * statistics. */
 PGB_API int pgb_paged_attention(const pgb_tensor *q, const pgb_tensor *k_cache, const pgb_tensor *v_cache,
                                 const pgb_tensor *k_scale, const pgb_tensor *v_scale, const pgb_tensor *q_start,

@@ -55,7 +55,8 @@ static int paged_attention(const pgb_tensor *q, const pgb_tensor *k_cache, const
   // Rows of a sequence on average, times the query heads that share a key: what rides on one pass over the keys. Both kernels
   // are right for any number; the one of 16-row tiles reads the keys again for every further 16. Of 16, 24 and 64 such rows
   // it takes 56, 85 and 175 us, the one of 256-row tiles 63, 64 and 66 (64 sequences of 500 tokens, 12 heads of 64); beside
-  // 8 int8 contexts of 2000 it takes 48, 62 and 71 against 65, 65 and 66.
+  // 8 int8 contexts of 2000 it takes 48, 62 and 71 against 65, 65 and 66. Longer contexts and head dim 128 cross later (8 int8 contexts
+  // of 4000, 32 heads of 128 on 8: 16 rows take 54 us here, 20 rows 102 there); no rule on the rows alone fits all of them.
   if (a.rows * a.group > 16LL * p.n_seq && run_paged_chunk(a, c, p, q->dtype == PGB_F16, stream, &st)) return st;
   return run_paged_rows(a, c, p, q->dtype == PGB_F16, stream);
 }
