@@ -84,7 +84,7 @@ __device__ __forceinline__ uint2 ld_shared8(uint32_t a) {
 }
 template <bool HALF, int D, bool I8>
 __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::kCtas) paged_rows_kernel(const __grid_constant__ PagedParams a, const __grid_constant__ KvCache c,
-                                                                       const __grid_constant__ KvPlan p, unsigned splits, unsigned tiles_per_token) {
+                                                                       const __grid_constant__ KvPlan p, unsigned splits, unsigned tiles_per_token, int by_slot) {
   using S = RowTile<D, I8>;
   constexpr int kRowWarps = S::kWarps;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -94,12 +94,30 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
   const int kvh = (int)(unit % c.heads);
   unit /= c.heads;
   const int sub = (int)(unit % tiles_per_token);  // which 16 query heads, where more than that share a key head
-  const int64_t row0 = unit / tiles_per_token;
-  const int seq = kv_sequence(p, row0);
-  if (seq < 0) return;
-  const int64_t first = __ldg(p.start + seq), end = min((int64_t)__ldg(p.start + seq + 1), a.rows);
   const int tokens = a.group >= 16 ? 1 : 16 / a.group;  // tokens of a tile
-  if ((row0 - first) % tokens) return;                 // another tile's row
+  // One tile for each row (with one new token per sequence), of which those return that begin none; or one for each slot:
+  // the slots of sequence s begin at start[s] / tokens + s, and it has at least as many as tiles.
+  int64_t row0 = unit / tiles_per_token, first;
+  int seq;
+  if (by_slot) {
+    const int64_t slot = row0;
+    int hi = p.n_seq;
+    seq = 0;
+    while (hi - seq > 1) {
+      const int mid = (seq + hi) >> 1;
+      if (__ldg(p.start + mid) / tokens + mid <= slot) seq = mid;
+      else hi = mid;
+    }
+    first = __ldg(p.start + seq);
+    row0 = first + (slot - first / tokens - seq) * tokens;
+  } else {
+    seq = kv_sequence(p, row0);
+    if (seq < 0) return;
+    first = __ldg(p.start + seq);
+    if ((row0 - first) % tokens) return;  // another tile's row
+  }
+  const int64_t end = min((int64_t)__ldg(p.start + seq + 1), a.rows);
+  if (first < 0 || row0 < first || row0 >= end) return;
   // Row i of the tile: token i / group, query head i % group (of the 16 that start at sub * 16)
   const int heads_here = min(a.group - sub * 16, 16);
   const int n_tok = (int)min((int64_t)tokens, end - row0);
@@ -514,7 +532,7 @@ __global__ void __launch_bounds__(RowTile<D, I8>::kWarps * 32, RowTile<D, I8>::k
 }
 
 template <bool HALF, int D, bool I8>
-static int launch(const PagedParams &a, const KvCache &c, const KvPlan &p, int splits, int tiles_per_token, int64_t units, cudaStream_t stream) {
+static int launch(const PagedParams &a, const KvCache &c, const KvPlan &p, int splits, int tiles_per_token, bool by_slot, int64_t units, cudaStream_t stream) {
   using S = RowTile<D, I8>;
   const auto kernel = paged_rows_kernel<HALF, D, I8>;
   // the attribute belongs to the device: set once on each, again where two threads meet
@@ -539,7 +557,7 @@ static int launch(const PagedParams &a, const KvCache &c, const KvPlan &p, int s
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, c, p, (unsigned)splits, (unsigned)tiles_per_token);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, c, p, (unsigned)splits, (unsigned)tiles_per_token, by_slot ? 1 : 0);
   if (e != cudaSuccess) {
     cudaGetLastError();
     set_error(std::string("paged_rows_kernel: ") + cudaGetErrorString(e));
@@ -551,22 +569,25 @@ static int launch(const PagedParams &a, const KvCache &c, const KvPlan &p, int s
 
 int run_paged_rows(const PagedParams &a, const KvCache &c, const KvPlan &p, bool half, cudaStream_t stream) {
   const int tiles_per_token = (a.group + 15) / 16;
-  const int64_t units = a.rows * tiles_per_token * c.heads;
-  // A row that begins no tile has CTAs too, which return at once: it is the tiles that count below, of which each sequence that
-  // has rows adds at most one that is not full.
+  // Work is dealt out by rows or by slots, whichever are fewer (4 sequences of 4000 tokens, 16 heads of 128, 16 new tokens each: 77
+  // and 55 us). Some of either have nothing to do; the tiles, of which each sequence that has rows adds at most one that is not
+  // full, are what counts for the split.
   const int64_t tokens = a.group >= 16 ? 1 : 16 / a.group, k = p.n_seq < a.rows ? p.n_seq : a.rows;
+  const bool by_slot = a.rows / tokens + p.n_seq < a.rows;
+  const int64_t units = (by_slot ? a.rows / tokens + p.n_seq : a.rows) * tiles_per_token * c.heads;
   const int64_t tiles = ((a.rows - k) / tokens + k) * tiles_per_token * c.heads;
-  // As many CTAs per item as leave no SM idle, up to a portable cluster; not more than have a block of keys for each warp.
+  // As many CTAs per item as leave no SM idle, up to a portable cluster; not more than have a block of keys for each warp, or two
+  // where a tile has several tokens' rows to join (the same with 300 tokens: 25 us with one, 16 with two, 19 with four).
   int splits = 1;
   const int warps = c.head_dim == 64 ? 2 : 4;
   const int64_t blocks = ((int64_t)p.width << c.log2_page) / (c.head_dim == 64 ? 32 : 16);
-  while (splits < 8 && tiles * splits < 4LL * sm_count() && blocks > (int64_t)splits * warps) splits *= 2;
+  while (splits < 8 && tiles * splits < 4LL * sm_count() && blocks > (int64_t)splits * warps * (a.rows > p.n_seq ? 2 : 1)) splits *= 2;
   if (units * splits > 2147483647LL) {
     set_error("paged_attention: too many rows for one launch");
     return PGB_ERR_UNSUPPORTED;
   }
   const bool i8 = c.dtype == PGB_I8;
-#define PGB_ROWS(H, D, Q) return launch<H, D, Q>(a, c, p, splits, tiles_per_token, units, stream)
+#define PGB_ROWS(H, D, Q) return launch<H, D, Q>(a, c, p, splits, tiles_per_token, by_slot, units, stream)
   if (half) {
     if (c.head_dim == 64) { if (i8) PGB_ROWS(true, 64, true); PGB_ROWS(true, 64, false); }
     if (i8) PGB_ROWS(true, 128, true);

@@ -227,6 +227,29 @@ def test_a_few_tokens_over_long_contexts(new, ctx, dtype, cache, D, Hq, Hkv):
     assert (out[plan.starts[-1]:] == 7).all() and same(out[:plan.starts[-1]], attend(plan, q, c)[:plan.starts[-1]])
 
 
+@pytest.mark.parametrize("dtype,cache,D,Hq,Hkv", [(F16, F16, 64, 2, 2), (BF16, BF16, 128, 6, 2), (F16, I8, 64, 5, 1), (BF16, I8, 128, 16, 2), (F16, F16, 64, 15, 1)])
+def test_every_row_of_uneven_sequences_is_found(dtype, cache, D, Hq, Hkv):
+    """Numbers of new tokens around those of a tile, in every order, empty sequences between them, offsets that do not begin at
+    zero: the rows kernel deals its tiles out by slots of which some are empty, and every tile must have one."""
+    g = torch.Generator().manual_seed(5)
+    for case in range(12):
+        n = int(torch.randint(1, 40, (), generator=g))
+        new = torch.randint(0, (2, 4, 18, 34)[case % 4], (n,), generator=g).tolist()
+        limit = 16 * n * Hkv // Hq  # on average, for the rows kernel
+        while sum(new) > limit:
+            new[new.index(max(new))] //= 2
+        ctx = [x + int(torch.randint(0, 90, (), generator=g)) for x in new]
+        plan = Plan(new, ctx, 16, seed=case, pad_rows=3)
+        c = new_cache(plan, Hkv, D, cache)
+        q = randn(plan.rows, Hq, D, dtype=dtype, seed=case)
+        for skip in (0, 5):
+            plan.q_start = torch.tensor([s + skip for s in plan.starts], dtype=torch.int32, device="cuda")
+            out = torch.full((plan.rows + skip, Hq, D), 7.0, dtype=dtype, device="cuda")
+            attend(plan, torch.cat([q[:skip], q]), c, out=out)
+            check(plan, out[skip:], q, c)
+            assert (out[:skip] == 7).all() and (out[plan.starts[-1] + skip:] == 7).all()
+
+
 @pytest.mark.parametrize("new,nats", [(1, 14.5), (1, 18.0), (3, 18.0), (40, 14.5)])
 @pytest.mark.parametrize("dtype,cache,D", [(F16, F16, 64), (F16, I8, 64), (BF16, I8, 128), (F16, F16, 128)])
 def test_many_small_probabilities_beside_one_that_is_not(new, nats, dtype, cache, D):
