@@ -53,11 +53,15 @@ static int paged_attention(const pgb_tensor *q, const pgb_tensor *k_cache, const
   if (a.rows == 0 || p.n_seq == 0) return PGB_OK;
   if (c.n_pages == 0) p.width = 0;  // no page at all: no key for anyone, and nothing to point a load at
   // Rows of a sequence on average, times the query heads that share a key: what rides on one pass over the keys. Both kernels
-  // are right for any number; the one of 16-row tiles reads the keys again for every further 16. Of 16, 24 and 64 such rows
-  // it takes 56, 85 and 175 us, the one of 256-row tiles 63, 64 and 66 (64 sequences of 500 tokens, 12 heads of 64); beside
-  // 8 int8 contexts of 2000 it takes 48, 62 and 71 against 65, 65 and 66. Longer contexts and head dim 128 cross later (8 int8 contexts
-  // of 4000, 32 heads of 128 on 8: 16 rows take 54 us here, 20 rows 102 there); no rule on the rows alone fits all of them.
-  if (a.rows * a.group > 16LL * p.n_seq && run_paged_chunk(a, c, p, q->dtype == PGB_F16, stream, &st)) return st;
+  // are right for any number; the one of 16-row tiles reads the keys again for every further 16, the one of 256-row tiles takes
+  // as long for any number up to 256. In us, 16-row tiles and 256-row tiles, 20 and 32 such rows (alone they have 4 to 64 sequences):
+  //   16 bits, head dim 128:  4 x 300 tokens 26, 29 and 16, 16;  16 x 1000 100, 78 and 52, 52;  8 x 4000 (grouped) 95, 81 and 62, 65
+  //   16 bits, head dim 64:   4 x 300 12, 14 and 13, 13;  64 x 500 59, 61 and 63, 64;  4 x 4000 31, 52 and 45, 46
+  // Beside an int8 cache the large tiles' step is longer and the small tiles' bytes fewer; 20, 32 and 48 rows:
+  //   head dim 64:   4 x 300 12, 12, 14 and 18;  64 x 500 49, 52, 74 and 107;  4 x 4000 25, 41, 41 and 70
+  //   head dim 128:  16 x 1000 75, 64, 81 and 85;  8 x 4000 (grouped) 74, 73, 84 and 102;  but 4 x 1000 38, 40, 44 and 29
+  const int64_t few = c.dtype == PGB_I8 ? 48 : 16;
+  if (a.rows * a.group > few * p.n_seq && run_paged_chunk(a, c, p, q->dtype == PGB_F16, stream, &st)) return st;
   return run_paged_rows(a, c, p, q->dtype == PGB_F16, stream);
 }
 

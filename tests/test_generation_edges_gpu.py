@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 F16, BF16, I8 = torch.float16, torch.bfloat16, torch.int8
 
 # new tokens, contexts, heads: tiles of sixteen rows; chunks whose keys are split over a cluster; chunks that are not split
-SIZES = [([2, 3], [400, 700], 2), ([200], [700], 2), ([40] * 24, [520] * 24, 8)]
+SIZES = [([2, 3], [400, 700], 2), ([200], [700], 2), ([40] * 24, [520] * 24, 8), ([60] * 24, [520] * 24, 8)]
 
 
 def check_numbers(plan, q, cache, got):
@@ -28,7 +28,7 @@ def check_numbers(plan, q, cache, got):
 
 
 @pytest.mark.parametrize("dtype,cache,D", [(F16, F16, 64), (BF16, BF16, 128), (F16, I8, 64), (BF16, I8, 128)])
-@pytest.mark.parametrize("new,ctx", [([20] * 50, [0] * 50), ([300] * 20 + [20] * 30, [-5] * 50), ([100] * 24 + [20] * 60, [300] * 24 + [0] * 60), ([150] * 12 + [1] * 90, [260] * 12 + [0] * 90)])
+@pytest.mark.parametrize("new,ctx", [([20] * 50, [0] * 50), ([60] * 50, [0] * 50), ([300] * 20 + [20] * 30, [-5] * 50), ([100] * 24 + [20] * 60, [300] * 24 + [0] * 60), ([150] * 12 + [1] * 90, [260] * 12 + [0] * 90), ([150] * 12 + [50] * 90, [260] * 12 + [0] * 90)])
 def test_hundreds_of_work_items_without_a_key(new, ctx, dtype, cache, D):
     # several in a row for every CTA, alone and behind items with keys; with a table and without one
     H = 12
@@ -52,7 +52,7 @@ def test_hundreds_of_work_items_without_a_key(new, ctx, dtype, cache, D):
 @pytest.mark.parametrize("cache", [F16, I8])
 def test_waits_for_items_end_with_the_others(cache):
     # a launch that loads nothing and whose first items have no keys: roles that wait for items give up when nothing moves
-    plan = Plan([20] * 60 + [200] * 4, [0] * 60 + [200] * 4, 32)
+    plan = Plan([60] * 60 + [200] * 4, [0] * 60 + [200] * 4, 32)
     c = new_cache(plan, 12, 64, cache)
     q = randn(plan.rows, 12, 64)
     K.gemm_wait_drill(1 << 14, skip_loads=True)
@@ -250,7 +250,7 @@ def test_every_row_of_uneven_sequences_is_found(dtype, cache, D, Hq, Hkv):
             assert (out[:skip] == 7).all() and (out[plan.starts[-1] + skip:] == 7).all()
 
 
-@pytest.mark.parametrize("new,nats", [(1, 14.5), (1, 18.0), (3, 18.0), (40, 14.5)])
+@pytest.mark.parametrize("new,nats", [(1, 14.5), (1, 18.0), (3, 18.0), (40, 14.5), (60, 14.5)])
 @pytest.mark.parametrize("dtype,cache,D", [(F16, F16, 64), (F16, I8, 64), (BF16, I8, 128), (F16, F16, 128)])
 def test_many_small_probabilities_beside_one_that_is_not(new, nats, dtype, cache, D):
     """One key lies 14.5 or 18 above 60000 others: each has a probability of 2^-21 or 2^-26, and together they make 3 % or 0.1 %
