@@ -29,7 +29,8 @@
 // Bound by the latency of a softmax warp's chain (two warps a scheduler) more than by either pipe. A step of 256 rows and 128
 // keys takes 2.0 us with head dim 64 (610 TFLOP/s over the GPU, the tensor pipe at a fifth of its cycles in a profile),
 // 3.2 us with 128 (780 TFLOP/s; S waits for the product that reads P), 3.5 and 5 us beside an int8 cache, whose scales are
-// read twice a score, and for fp16 their exponents once (2 of 51 us for 10 steps). A launch and its first item cost 10 us before and behind the steps, each further item 4.
+// read twice a score, and for fp16 their exponents once (2 of 51 us for 10 steps). A launch and its first item cost 10 us before
+// and behind the steps, each further item 4.
 // Tried and slower: 128 scores held in registers (spills, 4.7 us a step with head dim 64, and the code leaves the instruction
 // cache); one MMA warp for both halves; every role searching its items itself (74 against 50 us for 8 x 1024 tokens); giving S
 // up with half of its exponentials to go instead of a quarter (no gain in 16 bits, 52 against 49 us beside an int8 cache).

@@ -12,10 +12,11 @@
 //   softmax  running maximum and sum per row in fp32; the warps' and then the CTAs' partial results are joined in shared and
 //            distributed shared memory, in a fixed order. No scratch in global memory, nothing shared between launches.
 //   int8     widened exactly to fp16; the key's scale multiplies its scores, the value's scale its probabilities, in fp32.
-// Measured: 16 sequences of up to 32768 int8 tokens, 32 heads of 128 on 8: 181 us, 3.4 TB/s, half the copy rate; 64 of up to
+// Measured: 16 sequences of up to 32768 int8 tokens, 32 heads of 128 on 8: 183 us, 3.4 TB/s, half the copy rate; 64 of up to
 // 1024 tokens, 12 heads of 64 in fp16: 38 us, 3.5 TB/s. What bounds them then is the latency of a warp's chain from copy to
-// second product, with the twelve warps whose registers fit an SM (eight, whose stages do, with 128 values of 16 bits). Tiles of 8 rows (half the output's registers) gave 176 and
-// 39 us, a cap at 128 registers for sixteen warps 329 (spills): neither is worth a second set of kernels.
+// second product, with the twelve warps whose registers fit an SM (eight, whose stages do, with 128 values of 16 bits). Tiles of
+// 8 rows (half the output's registers) gave 176 and 39 us, a cap at 128 registers for sixteen warps 329 (spills): neither is
+// worth a second set of kernels.
 #include <atomic>
 #include <string>
 #include <type_traits>
