@@ -8,14 +8,17 @@ namespace pgb {
 
 // A run of `len` bytes at `base`, repeated over up to four dims (strides in bytes, not negative).
 struct ByteView {
-  uintptr_t base = 0;
-  int64_t len = 0;
+  uintptr_t base;
+  int64_t len;
+  __int128 end;  // behind the last byte
   int dims = 0;
   int64_t n[4], stride[4];
 
+  ByteView(uintptr_t at = 0, int64_t bytes = 0) : base(at), len(bytes), end((__int128)at + bytes) {}
   void add(int64_t extent, int64_t step) {
     if (extent <= 0) len = 0;
     if (extent > 1) {
+      end += (__int128)(extent - 1) * step;
       n[dims] = extent;
       stride[dims++] = step;
     }
@@ -68,19 +71,13 @@ struct StrideSums {
 // Of a tensor descriptor whose last dim is contiguous, `es` bytes an element, up to five dims.
 template <typename Tensor>
 inline ByteView view_of(const Tensor &t, int es) {
-  ByteView v;
-  v.base = reinterpret_cast<uintptr_t>(t.data);
-  v.len = es * t.shape[t.ndim - 1];
+  ByteView v(reinterpret_cast<uintptr_t>(t.data), es * t.shape[t.ndim - 1]);
   for (int i = 0; i + 1 < t.ndim; ++i) v.add(t.shape[i], t.stride_bytes[i]);
   return v;
 }
 
 inline bool views_share(const ByteView &a, const ByteView &b) {
-  if (a.len <= 0 || b.len <= 0) return false;
-  __int128 a_end = (__int128)a.base + a.len, b_end = (__int128)b.base + b.len;
-  for (int i = 0; i < a.dims; ++i) a_end += (__int128)(a.n[i] - 1) * a.stride[i];
-  for (int i = 0; i < b.dims; ++i) b_end += (__int128)(b.n[i] - 1) * b.stride[i];
-  if (a_end <= (__int128)b.base || b_end <= (__int128)a.base) return false;  // the usual case
+  if (a.end <= (__int128)b.base || b.end <= (__int128)a.base || a.len <= 0 || b.len <= 0) return false;  // the usual case
   StrideSums d;
   for (int i = 0; i < a.dims; ++i) d.add(a.stride[i], 0, a.n[i] - 1);
   for (int i = 0; i < b.dims; ++i) d.add(b.stride[i], 1 - b.n[i], 0);

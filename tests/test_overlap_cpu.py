@@ -15,9 +15,7 @@ SHIM = """
 #include "overlap.hpp"
 using namespace pgb;
 static ByteView make(const int64_t *v) {
-  ByteView b;
-  b.base = (uintptr_t)v[0];
-  b.len = v[1];
+  ByteView b((uintptr_t)v[0], v[1]);
   for (int i = 0; i < v[2]; ++i) b.add(v[3 + 2 * i], v[4 + 2 * i]);
   return b;
 }
