@@ -91,11 +91,15 @@ class PagedKVCache:
         return dict(k_scale=None, v_scale=None) if self.k_scale is None else dict(k_scale=self.k_scale[i], v_scale=self.v_scale[i])
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, plan: KVPlan) -> None:
-        """Stores the step's keys and values [rows, heads, head dim] of one layer."""
+        """Stores the step's keys and values [rows, heads, head dim] of one layer. Rows behind the plan's are padding."""
+        if len(k) < plan.rows:
+            raise ValueError(f"write: {len(k)} rows for a plan of {plan.rows}")
         K.kv_write(k, v, self.k[layer], self.v[layer], plan.q_start, plan.ctx_len, plan.page_table, **self._layer(layer))
 
     def attend(self, layer: int, q: torch.Tensor, plan: KVPlan, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """Causal attention of the step's queries [rows, query heads, head dim] over all that is stored of their sequences."""
+        if len(q) < plan.rows:
+            raise ValueError(f"attend: {len(q)} rows for a plan of {plan.rows}")
         return K.paged_attention(q, self.k[layer], self.v[layer], plan.q_start, plan.ctx_len, plan.page_table, scale, out=out, **self._layer(layer))
 
     def read(self, layer: int, seqs: Sequence[int], out_dtype=None):

@@ -1,4 +1,4 @@
-"""Plans in which a sequence has no new token."""
+"""Plans in which a sequence has no new token, and steps with fewer rows than their plan."""
 import pytest
 import torch
 
@@ -19,3 +19,13 @@ def test_a_sequence_without_a_new_token_has_no_last_row():
     with pytest.raises(ValueError, match="no last row"):
         model.forward_cached(torch.zeros(2, dtype=torch.int32), c, p)
     assert c.extend([], []).fewest == 1  # a step of no sequences lacks no row
+
+
+def test_a_step_with_fewer_rows_than_its_plan_is_refused():
+    c = cache(8)
+    p = c.extend([c.open()], [5])
+    x = torch.zeros((4, 3, 64), dtype=torch.float16)
+    with pytest.raises(ValueError, match="4 rows for a plan of 5"):
+        c.write(0, x, x, p)
+    with pytest.raises(ValueError, match="4 rows for a plan of 5"):
+        c.attend(0, x, p)
