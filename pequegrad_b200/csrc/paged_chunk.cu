@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const __g
           mbar_arrive(&item_full[slot]);
         }
         __syncwarp();
-        if (!more || P.splits > 1) ok = given_up(slot, parity);  // the last of all items, or of this round: nobody waits for one after it
+        if (!more || P.splits > 1) ok = given_up(slot, parity);  // the last of all items, or of this pass: nobody waits for one after it
         if (P.splits > 1) {  // one between two joins
           ++taken;
           break;
